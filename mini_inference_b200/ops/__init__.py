@@ -9,6 +9,7 @@ of float32 sums whether they run as multiply-adds or as bfloat16 parts on the te
 """
 from __future__ import annotations
 
+import contextlib
 import ctypes
 import math
 import os
@@ -1696,6 +1697,92 @@ class CudaOps:
                                   out, self._stream()), "sample")
         self.launches += 1
         return out
+
+
+    # ---------------------------------------------------------------- beam search
+    MAX_CANDIDATES, MAX_BEAMS = 128, 100     # most candidates that beam_select gives a group; most rows of a group that reorder_rows takes
+
+    def _here(self, what, **tensors):
+        """That all tensors are on this device (the last check of arguments: it is the one that a call on the CPU cannot pass)."""
+        for name, t in tensors.items():
+            if t.device.type != "cuda" or t.device.index != self._device_index:
+                raise ValueError(f"{what}: {name} on {t.device}, these kernels run on cuda:{self._device_index}")
+
+    @staticmethod
+    def _plain(what, dtype, **tensors):
+        """That all tensors are contiguous and of one dtype."""
+        for name, t in tensors.items():
+            if t.dtype != dtype:
+                raise TypeError(f"{what}: {name} is {t.dtype}, expected {dtype}")
+            if not t.is_contiguous():
+                raise ValueError(f"{what}: {name} is not contiguous")
+
+    def _current(self):
+        """The device made current for a launch, where another one is."""
+        return contextlib.nullcontext() if torch.cuda.current_device() == self._device_index else torch.cuda.device(self._device_index)
+
+    def beam_select(self, logits, scores, group_start, num):
+        """A beam search step's candidates.  logits float32 [R, V] (rows may be strided), scores float32 [R]: a row per beam and the sum of
+        its tokens' log-probabilities so far; group_start int32 [G + 1]: the beams of prompt g are rows group_start[g] .. group_start[g + 1] - 1.  A
+        candidate (row, token) has the value score + log_softmax(logits[row])[token].  Returns (values float32, rows int32, tokens int32), each [G, num]
+        (num at most 128): the best of each group, best first; equal values: the lower row, then the larger logit, then the lower token.  Values are
+        compared in float64.  Tokens with a logit of -inf are no candidates, nor are rows whose logits hold NaN or +inf or nothing finite or whose
+        score is not finite; places that stay empty hold (-inf, -1, -1)."""
+        self._plain("beam_select", torch.float32, scores=scores)
+        self._plain("beam_select", torch.int32, group_start=group_start)
+        if logits.dtype != torch.float32:
+            raise TypeError(f"beam_select: logits are {logits.dtype}, expected torch.float32")
+        if logits.dim() != 2 or scores.dim() != 1 or scores.shape[0] != logits.shape[0] or group_start.dim() != 1 or group_start.shape[0] < 1:
+            raise ValueError(f"beam_select: logits {tuple(logits.shape)}, scores {tuple(scores.shape)} and group_start {tuple(group_start.shape)} do not fit together")
+        (R, V), G = logits.shape, group_start.shape[0] - 1
+        if not 1 <= num <= self.MAX_CANDIDATES:
+            raise ValueError(f"beam_select: {num} candidates a group, between 1 and {self.MAX_CANDIDATES} are possible")
+        if V < 1 or (V > 1 and logits.stride(1) != 1) or (R > 1 and logits.stride(0) < V):
+            raise ValueError(f"beam_select: logits of shape {tuple(logits.shape)} with strides {logits.stride()} (a row's logits lie side by side)")
+        self._here("beam_select", logits=logits, scores=scores, group_start=group_start)
+        dev = logits.device
+        values = torch.empty((G, num), dtype=torch.float32, device=dev)
+        rows, tokens = torch.empty((G, num), dtype=torch.int32, device=dev), torch.empty((G, num), dtype=torch.int32, device=dev)
+        with self._current():
+            n = int(self.lib.mi_beam_select_bytes(R, V, num))
+            if n < 0:
+                _check(n, "beam_select")
+            work = torch.empty(max(n, 16), dtype=torch.uint8, device=dev)
+            _check(self.lib.mi_beam_select(logits, logits.stride(0) if R > 1 else V, R, V, scores, group_start, G, num, values, rows, tokens, work, self._stream()),
+                   "beam_select")
+        self.launches += (2 if R else 1) if G else 0
+        return values, rows, tokens
+
+    def reorder_rows(self, tensors, rows, parents, group_start, most, dim=0):
+        """In place, for every tensor t of `tensors` and every i: t[rows[i]] = what t[rows[parents[i]]] was before the call (a beam takes over its parent's
+        state).  dim: which dimension of the tensors the rows are (those before it are as many tables with the same rows; tensors of any type, contiguous
+        from the rows' dimension on, and before it too).  rows, parents int32 [n]; group_start int32 [G + 1]: places group_start[g] .. group_start[g + 1] - 1 of
+        both lists are a group, parents (places in the lists) lie in their row's group; most: rows of the largest group, at most 100.  A row is named once.
+        A parent outside its group, or a row that a tensor does not have, leaves the row as it is."""
+        tensors = list(tensors)
+        self._plain("reorder_rows", torch.int32, rows=rows, parents=parents, group_start=group_start)
+        if rows.dim() != 1 or rows.shape != parents.shape or group_start.dim() != 1 or group_start.shape[0] < 1:
+            raise ValueError(f"reorder_rows: rows {tuple(rows.shape)}, parents {tuple(parents.shape)} and group_start {tuple(group_start.shape)} do not fit together")
+        if not 0 <= most <= self.MAX_BEAMS:
+            raise ValueError(f"reorder_rows: groups of up to {most} rows, at most {self.MAX_BEAMS} are possible")
+        places = []
+        for t in tensors:
+            if not 0 <= dim < t.dim():
+                raise ValueError(f"reorder_rows: a tensor of shape {tuple(t.shape)} has no dimension {dim}")
+            size, n = t.element_size(), t.shape[dim]
+            row = math.prod(t.shape[dim + 1:])
+            stride = t.stride(dim) if n > 1 else row
+            if not t.is_contiguous() and (dim or not t[:1].is_contiguous() or stride < row):
+                raise ValueError(f"reorder_rows: a tensor of shape {tuple(t.shape)} has strides {t.stride()} (rows lie in one piece)")
+            places += (t.data_ptr(), math.prod(t.shape[:dim]), n * stride * size, n, stride * size, row * size)
+        self._here("reorder_rows", rows=rows, parents=parents, group_start=group_start, **{f"tensor {i}": t for i, t in enumerate(tensors)})
+        if places:
+            table = torch.tensor(places, dtype=torch.int64)
+            with self._current():
+                done = self.lib.mi_reorder_rows(table, len(tensors), rows, parents, group_start, group_start.shape[0] - 1, rows.shape[0], int(most), self._stream())
+            if done < 0:
+                _check(done if done > -1000 else -1000 - done, "reorder_rows")
+            self.launches += done
 
 
 _OPS = {}
