@@ -13,6 +13,7 @@ import contextlib
 import ctypes
 import math
 import os
+import types
 
 import torch
 
@@ -43,7 +44,6 @@ def load_calls():
     the same through ctypes."""
     global _CALLS
     if _CALLS is None:
-        import types
         from .build import INTEGER, POINTER, host_calls, signatures
         lib, fast, calls = load_library(), host_calls(), types.SimpleNamespace()
         for name, (ret, args) in signatures().items():
@@ -617,6 +617,9 @@ class CudaOps:
             self.launches += 1
         if not num_decode:
             return out
+        if not win and not split_weights and getattr(meta, "shared_start", None) is not None and self._takes_shared(q, k_cache, v_cache, meta, H, KV, D):
+            self._shared_decode(q, k_cache, v_cache, out, meta, H, KV, D, scale)
+            return out
         fast_decode = fast and H // KV <= 16 and meta.page_size % 16 == 0
         S = self.choose_splits(num_decode * (KV if fast_decode else math.ceil(H / 4)), meta.max_kv_len,
                                (2 if self.bulk_decode else 3) if fast_decode else 2,
@@ -652,6 +655,64 @@ class CudaOps:
                 H, KV, D, meta.page_size, S, scale, win, code, self._stream()), "attn_decode")
             self.launches += 2 if S > 1 else 1
         return out
+
+    def shared_prefix_attention(self, q, k_cache, v_cache, meta, H, KV, D, scale):
+        """Decode attention of rows whose caches begin with the same keys (beams or samples of a prompt): a group's prefix is read once for all its rows.
+        q [T, H D] (rows may be strided), caches [pages, KV, page_size, D].  meta: decode_segs int32 [R] (the entries, one fed token each), seg_q_start, seg_kv_len,
+        block_table and table_rows as paged_attention reads them (max_kv_len: the longest); shared_start int32 [G + 1]: entries decode_segs[shared_start[g]] ..
+        decode_segs[shared_start[g + 1] - 1] are group g (rows in no group stand alone), shared_len int32 [G]: the first so many keys of its rows are the
+        same, and are read by the pages of the first row that has them all; max_shared_rows, on the host: rows of the largest group (rows beyond it are computed alone).  An entry
+        without keys gets zeros.  The output [T, H D] has the entries' rows; others are left as they come.
+        Heads of 64 or 128 run on kernels that share; other heads, more than 4,096 entries and groups, and bfloat16 pages that neither divide 64 keys
+        nor are divided by them are computed row by row, by the rows' own pages."""
+        if q.dim() != 2 or q.shape[1] != H * D or H < 1 or KV < 1 or H % KV or (q.shape[1] > 1 and q.stride(1) != 1):
+            raise ValueError(f"shared_prefix_attention: queries {tuple(q.shape)} with strides {q.stride()} are no rows of {H} heads of {D} over {KV} key heads")
+        if k_cache.shape != v_cache.shape or k_cache.dim() != 4 or tuple(k_cache.shape[1:]) != (KV, meta.page_size, D):
+            raise ValueError(f"shared_prefix_attention: caches {tuple(k_cache.shape)} and {tuple(v_cache.shape)} are not [pages, {KV}, {meta.page_size}, {D}]")
+        if not scale > 0:
+            raise ValueError(f"shared_prefix_attention: scale {scale} is not positive")
+        if _code(q.dtype) != _code(k_cache.dtype) or k_cache.dtype != v_cache.dtype:
+            raise TypeError(f"shared_prefix_attention: queries {q.dtype}, caches {k_cache.dtype} and {v_cache.dtype}")
+        lists = dict(decode_segs=meta.decode_segs, seg_q_start=meta.seg_q_start, seg_kv_len=meta.seg_kv_len, shared_start=meta.shared_start, shared_len=meta.shared_len)
+        if getattr(meta, "table_rows", None) is not None:
+            lists["table_rows"] = meta.table_rows
+        self._plain("shared_prefix_attention", torch.int32, block_table=meta.block_table, **lists)
+        self._plain("shared_prefix_attention", k_cache.dtype, k_cache=k_cache, v_cache=v_cache)
+        if any(t.dim() != 1 for t in lists.values()) or meta.shared_start.shape[0] != meta.shared_len.shape[0] + 1:
+            raise ValueError(f"shared_prefix_attention: shared_start {tuple(meta.shared_start.shape)} and shared_len {tuple(meta.shared_len.shape)} do not fit together")
+        if meta.block_table.dim() != 2 or meta.block_table.shape[1] != meta.max_pages:
+            raise ValueError(f"shared_prefix_attention: block_table {tuple(meta.block_table.shape)} has no {meta.max_pages} pages a row")
+        self._here("shared_prefix_attention", q=q, k_cache=k_cache, v_cache=v_cache, block_table=meta.block_table, **lists)
+        with self._current():
+            if not self._takes_shared(q, k_cache, v_cache, meta, H, KV, D):
+                alone = types.SimpleNamespace(prefill_tiles=meta.decode_segs[:0].view(0, 2), tile=self.prefill_tile, max_kv_len=meta.max_kv_len, max_pages=meta.max_pages,
+                                              page_size=meta.page_size, block_table=meta.block_table, table_rows=getattr(meta, "table_rows", None), shared_start=None,
+                                              **{k: lists[k] for k in ("decode_segs", "seg_q_start", "seg_kv_len")})
+                return self.paged_attention(q, k_cache, v_cache, alone, H, KV, D, scale, None)
+            out = torch.empty((q.shape[0], H * D), dtype=q.dtype, device=q.device)
+            self._shared_decode(q, k_cache, v_cache, out, meta, H, KV, D, scale)
+        return out
+
+    def _takes_shared(self, q, k_cache, v_cache, meta, H, KV, D):
+        """Whether a kernel that reads shared prefixes once takes these rows."""
+        if not self.fast_attention or q.stride(0) % (16 // q.element_size()) or (q.data_ptr() | k_cache.data_ptr() | v_cache.data_ptr()) % 16:
+            return False
+        return self._shared_bytes(q, meta, H, KV, D) > 0
+
+    def _shared_bytes(self, q, meta, H, KV, D):
+        size = self.lib.mi_attn_shared_tc_bytes if q.dtype == torch.bfloat16 else self.lib.mi_attn_shared_f32_bytes
+        return int(size(meta.decode_segs.shape[0], meta.shared_len.shape[0], meta.max_shared_rows, H, KV, D, meta.page_size))
+
+    def _shared_decode(self, q, k_cache, v_cache, out, meta, H, KV, D, scale):
+        work = torch.empty(self._shared_bytes(q, meta, H, KV, D), dtype=torch.uint8, device=q.device)
+        rows = (out, meta.decode_segs, meta.decode_segs.shape[0], meta.seg_q_start, meta.seg_kv_len, meta.block_table, getattr(meta, "table_rows", None), meta.max_pages,
+                meta.shared_start, meta.shared_len, meta.shared_len.shape[0], meta.max_shared_rows, H, KV, D, meta.page_size, scale, work)
+        if q.dtype == torch.bfloat16:
+            _check(self.lib.mi_attn_shared_tc(q, q.stride(0), k_cache, v_cache, k_cache.shape[0] * KV * meta.page_size, *rows, self._stream_error, self._stream()),
+                   "attn_shared_tc")
+        else:
+            _check(self.lib.mi_attn_shared_f32(q, q.stride(0), k_cache, v_cache, *rows, self._stream()), "attn_shared_f32")
+        self.launches += 2
 
     # Where split softmax weights run on tcgen05: a prompt portion sees (first) so many keys, or 256 in a step of (second) so many tokens.  On the
     # device that form is the faster one at every point of 2 to 2,048 rows x 256 to 8,192 keys (256 keys: 8 us against 16, 2,048: 40 against 108); but its
@@ -1706,7 +1767,7 @@ class CudaOps:
         """That all tensors are on this device (the last check of arguments: it is the one that a call on the CPU cannot pass)."""
         for name, t in tensors.items():
             if t.device.type != "cuda" or t.device.index != self._device_index:
-                raise ValueError(f"{what}: {name} on {t.device}, these kernels run on cuda:{self._device_index}")
+                raise ValueError(f"{what}: {name} is on {t.device}, these kernels run on cuda:{self._device_index}")
 
     @staticmethod
     def _plain(what, dtype, **tensors):

@@ -46,3 +46,40 @@ class BeamRefOps(TorchRefOps):
 
     def reorder_rows(self, tensors, rows, parents, group_start, most, dim=0):
         reorder_rows_plain(tensors, rows, parents, group_start, dim)
+
+
+def shared_prefix_attention64(q, k_cache, v_cache, meta, H, KV, D, scale):
+    """(output, sum of weights times |values|, largest sum of |q k| scale) of the entries' rows in float64, by row: keys below its group's shared length by
+    the pages of the group's first row that has them all, the others by its own."""
+    R, ps, Hg = meta.decode_segs.shape[0], meta.page_size, H // KV
+    starts, shared = meta.shared_start.tolist(), meta.shared_len.tolist()
+    segs, toks, lens = meta.decode_segs.tolist(), meta.seg_q_start.tolist(), meta.seg_kv_len.tolist()
+    rows = list(range(len(lens))) if getattr(meta, "table_rows", None) is None else meta.table_rows.tolist()
+    table, k64, v64 = meta.block_table.cpu(), k_cache.cpu().double(), v_cache.cpu().double()
+    out = torch.zeros(q.shape[0], H * D, dtype=torch.float64)
+    size, reach = torch.zeros_like(out), 0.0
+    for r in range(R):
+        n, tok = lens[segs[r]], toks[segs[r]]
+        if n <= 0:
+            continue
+        g = next((g for g in range(len(shared)) if starts[g] <= r < starts[g + 1]), None)
+        key = torch.arange(n)
+        own = table[rows[segs[r]]][key // ps].long()
+        if g is not None:
+            holds = next((i for i in range(starts[g], starts[g + 1]) if lens[segs[i]] >= shared[g]), starts[g])
+            own = torch.where(key < shared[g], table[rows[segs[holds]]][key // ps].long(), own)
+        k, v = k64[own, :, key % ps], v64[own, :, key % ps]                       # [n, KV, D]
+        qr = q[tok].cpu().double().view(KV, Hg, D)
+        s = torch.einsum("khd,nkd->khn", qr, k) * scale
+        reach = max(reach, float((torch.einsum("khd,nkd->khn", qr.abs(), k.abs()) * scale).max()))
+        w = torch.softmax(s, dim=-1)
+        out[tok] = torch.einsum("khn,nkd->khd", w, v).reshape(-1)
+        size[tok] = torch.einsum("khn,nkd->khd", w, v.abs()).reshape(-1)
+    return out, size, reach
+
+
+def _shared_prefix_attention(self, q, k_cache, v_cache, meta, H, KV, D, scale):
+    return shared_prefix_attention64(q, k_cache, v_cache, meta, H, KV, D, scale)[0].to(q.device, q.dtype)
+
+
+BeamRefOps.shared_prefix_attention = _shared_prefix_attention
