@@ -65,10 +65,10 @@ __global__ void __launch_bounds__(THREADS, 2) attn_shared_f32_kernel(const __gri
         for (int id = tid; id < rows * PIECES; id += THREADS) {
             const int row = id / PIECES, c = id % PIECES * 4, r = walk.row0 + row / Hg, h = walk.kvh * Hg + row % Hg;
             *reinterpret_cast<float4*>(smem + T::Q + row * T::QS + c) =
-                *reinterpret_cast<const float4*>(q + (size_t)a.seg_q_start[a.decode_segs[r]] * q_stride + (size_t)h * D + c);
+                *reinterpret_cast<const float4*>(q + (size_t)plan.token[r] * q_stride + (size_t)h * D + c);
         }
         const int my_row = tid >> 3;                 // softmax: eight threads a row
-        const int hi = my_row < rows ? min(walk.hi, row_keys(a, walk.row0 + my_row / Hg)) : 0;
+        const int hi = my_row < rows ? min(walk.hi, plan.keys[walk.row0 + my_row / Hg]) : 0;
         float m = -INFINITY, l = 0.f, acc[4][C];
 #pragma unroll
         for (int i = 0; i < 4; ++i)
@@ -146,13 +146,14 @@ __global__ void __launch_bounds__(THREADS, 2) attn_shared_f32_kernel(const __gri
             }
             __syncthreads();                         // the stage, the scores and (behind the last tile) the queries are free
         }
-        const size_t at = (size_t)walk.place() * (walk.prefix ? a.slot_rows : Hg);
-        float* o = (walk.prefix ? a.o_prefix : a.o_tail) + (at + 4 * warp) * D + C * lane;
+        const int rows_of = walk.prefix ? a.slot_rows : Hg;
+        const size_t at = (size_t)walk.place() * rows_of;
+        float* o = (walk.prefix ? a.o_prefix : a.o_tail) + at * D + (C * lane / 4 * rows_of + 4 * warp) * 4 + C * lane % 4;
 #pragma unroll
         for (int r = 0; r < 4; ++r)
             if (4 * warp + r < rows) {
-                store2(o + r * D, acc[r][0], acc[r][1]);
-                if constexpr (C == 4) store2(o + r * D + 2, acc[r][2], acc[r][3]);
+                store2(o + 4 * r, acc[r][0], acc[r][1]);
+                if constexpr (C == 4) store2(o + 4 * r + 2, acc[r][2], acc[r][3]);
             }
         if (my_row < rows && (tid & 7) == 0) (walk.prefix ? a.ml_prefix : a.ml_tail)[at + my_row] = make_float2(m, l);
     }
@@ -187,11 +188,11 @@ MI_EXPORT int mi_attn_shared_f32(const float* q, int q_stride, const float* k_ca
     place_scratch(a, scratch(R, G, H, KV, D, a.row_tiles, a.slot_rows, blocks), work);
     const float scale_log2 = scale * 1.4426950408889634f;
 #define LAUNCH(DD) do { \
-        const size_t smem = (size_t)Tiles<DD>::END * 4, plan = (size_t)shared_plan_ints(G, R) * 4; \
-        cudaError_t e = cudaFuncSetAttribute(attn_shared_f32_kernel<DD>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)(smem + (3 * MAX_ENTITIES + 1) * 4)); \
+        const size_t smem = (size_t)Tiles<DD>::END * 4, plan = (size_t)plan_ints(G, R) * 4; \
+        cudaError_t e = cudaFuncSetAttribute(attn_shared_f32_kernel<DD>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)(smem + (6 * MAX_ENTITIES + 1) * 4)); \
         if (e == cudaSuccess) e = launch_pdl(attn_shared_f32_kernel<DD>, dim3(blocks), dim3(THREADS), smem + plan, stream, a, q, (long long)q_stride, k_cache, v_cache, \
                                              scale_log2); \
-        if (e == cudaSuccess) e = launch_pdl(merge_kernel<float, DD, KT>, dim3(R, KV), dim3(128), 0, stream, a, out); \
+        if (e == cudaSuccess) e = launch_pdl(merge_kernel<float, DD>, dim3(R, KV), dim3(128 * MERGE_PARTS), 0, stream, a, out); \
         return (int)e; \
     } while (0)
     if (D == 128) LAUNCH(128);

@@ -10,7 +10,7 @@
 //              there (what lies in a page's unused part may be anything, and 0 * inf is no 0) and handed on.
 //   warp 1     one thread issues S = Q K^T (scores in one of two 64-column buffers of tensor memory) a tile ahead, and O += P V
 //   warps 2-5  a matrix row a thread: mask, running maximum and sum (float32, base 2; the exponent's offset is kept until the maximum has grown by 2^8),
-//              weights as bfloat16 back to tensor memory.  With the last tile's weights handed over they bring the next piece's queries, then write
+//              weights as bfloat16 back to tensor memory; values that no row sees are cleared in shared memory.  With the last tile's weights handed over they bring the next piece's queries, then write
 //              this one's O, maximum and sum.  A warp whose 32 rows are all beyond the piece only keeps step.
 // Weights are rounded to bfloat16 for P V (2^-9 of each, of random sign over the keys; the sums take them unrounded), as the engine's other decode and prompt attention does.
 // Two launches: this one, and the merge.  Every mbarrier wait is bounded.
@@ -30,6 +30,17 @@ namespace {
 constexpr int BQ = 128, KT = 64, THREADS = 224;
 constexpr float LOG2E = 1.4426950408889634f;
 
+__device__ __forceinline__ float max3(float a, float b, float c) {      // one instruction on this architecture
+    float d;
+    asm("max.f32 %0, %1, %2, %3;\n" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+    return d;
+}
+__device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t (&r)[16]) {       // tmem_st32 for 16 columns
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};\n"
+                 :: "r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]),
+                    "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
+                 : "memory");
+}
 __device__ __forceinline__ uint32_t pack_bf16(float a, float b) {
     __nv_bfloat162 v = __floats2bfloat162_rn(a, b);
     return *reinterpret_cast<uint32_t*>(&v);
@@ -51,7 +62,7 @@ attn_shared_tc_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_con
     const uint32_t sQ = smem_u32(base), sK = sQ + Q_BYTES, sV = sK + 2 * KV_BYTES;
     const uint32_t q_full = smem_u32(bars), k_full = smem_u32(bars + 1), k_empty = smem_u32(bars + 3), s_full = smem_u32(bars + 5),
                    p_ready = smem_u32(bars + 7), pv_done = smem_u32(bars + 8), v_full = smem_u32(bars + 9), v_empty = smem_u32(bars + 11),
-                   v_ragged = smem_u32(bars + 13), o_free = smem_u32(bars + 14);
+                   o_free = smem_u32(bars + 13);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int Hg = a.H / a.KV;
 
@@ -59,7 +70,7 @@ attn_shared_tc_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_con
         mbar_init(q_full, 128);
         mbar_init(k_full, 1); mbar_init(k_full + 8, 1); mbar_init(k_empty, 1); mbar_init(k_empty + 8, 1);
         mbar_init(v_full, 1); mbar_init(v_full + 8, 1); mbar_init(v_empty, 1); mbar_init(v_empty + 8, 1);
-        mbar_init(s_full, 1); mbar_init(s_full + 8, 1); mbar_init(p_ready, 128); mbar_init(pv_done, 1); mbar_init(v_ragged, 1); mbar_init(o_free, 128);
+        mbar_init(s_full, 1); mbar_init(s_full + 8, 1); mbar_init(p_ready, 128); mbar_init(pv_done, 1); mbar_init(o_free, 128);
         mbar_init_fence();
         tma_prefetch_desc(&kmap); tma_prefetch_desc(&vmap);
     }
@@ -81,36 +92,22 @@ attn_shared_tc_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_con
         const uint32_t full = is_v ? v_full : k_full, empty = is_v ? v_empty : k_empty, dst0 = is_v ? sV : sK;
         const CUtensorMap* map = is_v ? &vmap : &kmap;
         bool ok = true;
-        int n = 0, cleared = 0;                              // tiles so far, of them cleared
+        int n = 0;                                           // tiles so far
         while (ok && walk.next()) {
             const int* table = walk.table();
             for (int i = 0; i < walk.tiles && ok; ++i, ++n) {
                 const int s = n & 1, key = walk.key0 + i * KT;
-                const int seen0 = max(0, walk.lo - key), seen1 = min(KT, walk.hi - key);      // the tile's visible keys
-                const bool ragged = is_v && (seen0 > 0 || seen1 < KT);
-                const uint32_t there = ragged ? v_ragged : full + 8 * s;
                 if (lane == 0) {
                     if (n >= 2 && !mbar_wait(empty + 8 * s, ((n >> 1) - 1) & 1)) { atomicExch(error_word, 61); ok = false; }
-                    if (ok) mbar_expect_tx(there, KV_BYTES);
+                    if (ok) mbar_expect_tx(full + 8 * s, KV_BYTES);
                 }
                 ok = __shfl_sync(0xffffffffu, ok, 0);
                 if (!ok) break;
                 for (int op = lane; op < ops_per_tile; op += 32) {
                     const int b = op / HALVES, hb = op % HALVES, j = key + b * box;
                     const int page = j < walk.hi ? table[j / a.ps] : 0;                        // behind the last key: the null page
-                    tma_load_2d(dst0 + s * KV_BYTES + hb * (KT * 128) + b * box * 128, map, hb * 64, (page * a.KV + walk.kvh) * a.ps + j % a.ps, there);
+                    tma_load_2d(dst0 + s * KV_BYTES + hb * (KT * 128) + b * box * 128, map, hb * 64, (page * a.KV + walk.kvh) * a.ps + j % a.ps, full + 8 * s);
                 }
-                if (!ragged) continue;
-                if (!__all_sync(0xffffffffu, mbar_spin(v_ragged, cleared & 1))) { if (lane == 0) atomicExch(error_word, 62); ok = false; break; }
-                ++cleared;
-                unsigned char* v = base + Q_BYTES + 2 * KV_BYTES + s * KV_BYTES;
-                for (int id = lane; id < KT * HALVES * 8; id += 32) {
-                    const int chunk = id % 8, hb = id / 8 % HALVES, vr = id / (8 * HALVES);
-                    if (vr < seen0 || vr >= seen1) *reinterpret_cast<uint4*>(v + hb * (KT * 128) + vr * 128 + chunk * 16) = make_uint4(0, 0, 0, 0);
-                }
-                asm volatile("fence.proxy.async.shared::cta;\n" ::: "memory");
-                __syncwarp();
-                if (lane == 0) mbar_arrive(v_full + 8 * s);
             }
         }
     } else if (warp == 1) {
@@ -122,7 +119,7 @@ attn_shared_tc_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_con
             int n = 0, pieces = 0;
             auto issue_qk = [&](int m) {
                 const int s = m & 1;
-                if (!mbar_spin(k_full + 8 * s, (m >> 1) & 1)) { atomicExch(error_word, 63); ok = false; return; }
+                if (!mbar_wait(k_full + 8 * s, (m >> 1) & 1)) { atomicExch(error_word, 63); ok = false; return; }
                 tc_fence_after();
 #pragma unroll
                 for (int ks = 0; ks < D / 16; ++ks) {
@@ -133,15 +130,15 @@ attn_shared_tc_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_con
                 umma_commit(s_full + 8 * s);
             };
             while (ok && walk.next()) {
-                if (!mbar_spin(q_full, pieces & 1)) { atomicExch(error_word, 64); break; }
+                if (!mbar_wait(q_full, pieces & 1)) { atomicExch(error_word, 64); break; }
                 issue_qk(n);
                 for (int i = 0; i < walk.tiles && ok; ++i, ++n) {
                     const int s = n & 1;
                     if (i + 1 < walk.tiles) issue_qk(n + 1);       // a tile ahead of the softmax, within a piece
                     if (!ok) break;
-                    if (!mbar_spin(p_ready, n & 1)) { atomicExch(error_word, 65); ok = false; break; }
-                    if (!mbar_spin(v_full + 8 * s, (n >> 1) & 1)) { atomicExch(error_word, 66); ok = false; break; }
-                    if (i == 0 && pieces > 0 && !mbar_spin(o_free, (pieces - 1) & 1)) { atomicExch(error_word, 67); ok = false; break; }
+                    if (!mbar_wait(p_ready, n & 1)) { atomicExch(error_word, 65); ok = false; break; }
+                    if (!mbar_wait(v_full + 8 * s, (n >> 1) & 1)) { atomicExch(error_word, 66); ok = false; break; }
+                    if (i == 0 && pieces > 0 && !mbar_wait(o_free, (pieces - 1) & 1)) { atomicExch(error_word, 67); ok = false; break; }
                     tc_fence_after();
 #pragma unroll
                     for (int kk = 0; kk < KT / 16; ++kk)
@@ -156,11 +153,21 @@ attn_shared_tc_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_con
         // ---------------- softmax: thread <-> (row, head) <-> tensor-memory lane
         const int lg = warp & 3, mine = lg * 32 + lane, tid = threadIdx.x - 64;
         const uint32_t lane_addr = tmem + ((uint32_t)(lg * 32) << 16);
-        auto bring_queries = [&](const Walk<KT>& w) {          // the piece's queries into swizzled rows of shared memory
-            for (int id = tid; id < w.rows * Hg * (D / 8); id += 128) {
-                const int row = id / (D / 8), c = id % (D / 8), r = w.row0 + row / Hg, h = w.kvh * Hg + row % Hg;
-                const uint4 v = *reinterpret_cast<const uint4*>(q + (size_t)a.seg_q_start[a.decode_segs[r]] * q_stride + (size_t)h * D + c * 8);
-                *reinterpret_cast<uint4*>(base + (c / 8) * (BQ * 128) + row * 128 + (((c % 8) ^ (row & 7)) << 4)) = v;
+        auto bring_queries = [&](const Walk<KT>& w) {          // the piece's queries into swizzled rows of shared memory, eight pieces of 16 bytes of a thread in flight
+            constexpr int C = D / 8, STEP = 128 / C;
+            const int c = tid % C, first = tid / C, n = w.rows * Hg;
+            for (int row0 = first; row0 < n; row0 += 8 * STEP) {
+                uint4 v[8];
+#pragma unroll
+                for (int k = 0; k < 8; ++k) {
+                    const int row = row0 + k * STEP;
+                    if (row < n) v[k] = *reinterpret_cast<const uint4*>(q + (size_t)plan.token[w.row0 + row / Hg] * q_stride + (size_t)(w.kvh * Hg + row % Hg) * D + c * 8);
+                }
+#pragma unroll
+                for (int k = 0; k < 8; ++k) {
+                    const int row = row0 + k * STEP;
+                    if (row < n) *reinterpret_cast<uint4*>(base + (c / 8) * (BQ * 128) + row * 128 + (((c % 8) ^ (row & 7)) << 4)) = v[k];
+                }
             }
             asm volatile("fence.proxy.async.shared::cta;\n" ::: "memory");
             mbar_arrive(q_full);
@@ -171,29 +178,36 @@ attn_shared_tc_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_con
         while (more && ok) {
             const int rows = walk.rows * Hg, tiles = walk.tiles, key0 = walk.key0, lo = walk.lo, place = walk.place();
             const bool prefix = walk.prefix, active = lg * 32 < rows;
-            // a prefix's rows see no further than their own length
-            const int hi = mine < rows ? min(walk.hi, row_keys(a, walk.row0 + mine / Hg)) : 0;
+            const int hi = walk.hi;
+            // a prefix's rows see no further than their own length; lanes beyond the rows hold anything
+            const int mine_hi = mine < rows ? min(hi, plan.keys[walk.row0 + mine / Hg]) : hi;
             float m_ref = -INFINITY, l = 0.f;
             for (int i = 0; i < tiles && ok; ++i, ++n) {
-                const uint32_t s_col = S_COL + 64 * (n & 1);
-                if (!mbar_spin(s_full + 8 * (n & 1), (n >> 1) & 1)) { atomicExch(error_word, 68); ok = false; break; }
+                const int s = n & 1, key = key0 + i * KT;
+                const uint32_t s_addr = lane_addr + S_COL + 64 * s;
+                if (!mbar_wait(s_full + 8 * s, (n >> 1) & 1)) { atomicExch(error_word, 68); ok = false; break; }
                 tc_fence_after();
                 float alpha = 1.f;
                 bool rescale = false;
                 if (active) {
-                    uint32_t r[64];
-                    tmem_ld32(lane_addr + s_col, *reinterpret_cast<uint32_t(*)[32]>(&r[0]));
-                    tmem_ld32(lane_addr + s_col + 32, *reinterpret_cast<uint32_t(*)[32]>(&r[32]));
-                    tmem_wait_ld();
-                    const int key = key0 + i * KT;
-                    if (!__all_sync(0xffffffffu, key >= lo && key + KT <= hi)) {
-#pragma unroll
-                        for (int c = 0; c < 64; ++c)
-                            if (key + c < lo || key + c >= hi) r[c] = 0xff800000u;      // -inf
-                    }
+                    // The scores in two halves of 32, read twice: for the maximum, and for the weights (few registers, little code)
+                    const bool whole = __all_sync(0xffffffffu, key >= lo && key + KT <= mine_hi);
+                    const uint32_t from = (uint32_t)(key - lo), span = (uint32_t)max(mine_hi - lo, 0);      // a key in front of lo wraps around
                     float mx4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+                    uint32_t r[32];
+#pragma unroll 1
+                    for (int half = 1; half >= 0; --half) {
+                        tmem_ld32(s_addr + 32 * half, r);
+                        tmem_wait_ld();
+                        if (!whole) {
 #pragma unroll
-                    for (int c = 0; c < 64; ++c) mx4[c & 3] = fmaxf(mx4[c & 3], __uint_as_float(r[c]));
+                            for (int c = 0; c < 32; ++c) r[c] = from + (half * 32 + c) < span ? r[c] : 0xff800000u;       // -inf
+                        }
+#pragma unroll
+                        for (int c = 0; c < 32; c += 8)
+#pragma unroll
+                            for (int e = 0; e < 4; ++e) mx4[e] = max3(mx4[e], __uint_as_float(r[c + 2 * e]), __uint_as_float(r[c + 2 * e + 1]));
+                    }
                     const float mx = fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3])) * scale_log2;      // scale > 0
                     if (mx > m_ref + 8.f) {
                         alpha = m_ref == -INFINITY ? 0.f : fast_exp2(m_ref - mx);
@@ -202,22 +216,43 @@ attn_shared_tc_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_con
                         l *= alpha;
                     }
                     const float off = m_ref == -INFINITY ? 0.f : m_ref;
-                    uint32_t pk[32];
                     const float2 scale2 = make_float2(scale_log2, scale_log2), noff2 = make_float2(-off, -off);
-                    float2 sums[4] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f), make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
+                    float2 sums[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
+#pragma unroll 1
+                    for (int half = 0; half < 2; ++half) {             // r holds the first half
+                        if (half) {
+                            tmem_ld32(s_addr + 32, r);
+                            tmem_wait_ld();
+                            if (!whole) {
 #pragma unroll
-                    for (int c = 0; c < 32; ++c) {
-                        const float2 arg = __ffma2_rn(make_float2(__uint_as_float(r[2 * c]), __uint_as_float(r[2 * c + 1])), scale2, noff2);
-                        const float2 p = make_float2(fast_exp2(arg.x), fast_exp2(arg.y));
-                        sums[c & 3] = __fadd2_rn(sums[c & 3], p);
-                        pk[c] = pack_bf16(p.x, p.y);
+                                for (int c = 0; c < 32; ++c) r[c] = from + (32 + c) < span ? r[c] : 0xff800000u;
+                            }
+                        }
+                        uint32_t pk[16];
+#pragma unroll
+                        for (int c = 0; c < 16; ++c) {
+                            const float2 arg = __ffma2_rn(make_float2(__uint_as_float(r[2 * c]), __uint_as_float(r[2 * c + 1])), scale2, noff2);
+                            const float2 p = make_float2(fast_exp2(arg.x), fast_exp2(arg.y));
+                            sums[c & 1] = __fadd2_rn(sums[c & 1], p);
+                            pk[c] = pack_bf16(p.x, p.y);
+                        }
+                        tmem_st16(s_addr + 16 * half, pk);             // P takes the place of the first scores
                     }
-                    const float2 s01 = __fadd2_rn(sums[0], sums[1]), s23 = __fadd2_rn(sums[2], sums[3]);
-                    l += (s01.x + s01.y) + (s23.x + s23.y);
-                    tmem_st32(lane_addr + s_col, pk);                  // P takes the place of the scores it came from
+                    const float2 s01 = __fadd2_rn(sums[0], sums[1]);
+                    l += s01.x + s01.y;
+                }
+                if (key < lo || key + KT > hi) {
+                    // Values in front of the piece's first or behind its last key may be anything (a page's unused part), and 0 * inf is no 0
+                    if (!mbar_wait(v_full + 8 * s, (n >> 1) & 1)) { atomicExch(error_word, 62); ok = false; break; }
+                    unsigned char* v = base + Q_BYTES + 2 * KV_BYTES + s * KV_BYTES;
+                    for (int id = tid; id < KT * HALVES * 8; id += 128) {
+                        const int chunk = id % 8, hb = id / 8 % HALVES, vr = id / (8 * HALVES);
+                        if (key + vr < lo || key + vr >= hi) *reinterpret_cast<uint4*>(v + hb * (KT * 128) + vr * 128 + chunk * 16) = make_uint4(0, 0, 0, 0);
+                    }
+                    asm volatile("fence.proxy.async.shared::cta;\n" ::: "memory");
                 }
                 // every thread follows pv_done phase by phase; O holds the tile before this one completely after it
-                if (n > 0 && !mbar_spin(pv_done, (n - 1) & 1)) { atomicExch(error_word, 69); ok = false; }
+                if (n > 0 && !mbar_wait(pv_done, (n - 1) & 1)) { atomicExch(error_word, 69); ok = false; }
                 if (__any_sync(0xffffffffu, rescale)) {
                     tc_fence_after();
 #pragma unroll 1
@@ -238,11 +273,11 @@ attn_shared_tc_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_con
             // the last tile's scores are there, so nothing reads this piece's queries any more
             more = walk.next();
             if (more) bring_queries(walk);
-            if (!mbar_spin(pv_done, (n - 1) & 1)) { atomicExch(error_word, 70); break; }
+            if (!mbar_wait(pv_done, (n - 1) & 1)) { atomicExch(error_word, 70); break; }
             tc_fence_after();
             if (active) {
-                const size_t row = (size_t)place * (prefix ? a.slot_rows : Hg) + mine;
-                float* orow = (prefix ? a.o_prefix : a.o_tail) + row * D;
+                const int rows_of = prefix ? a.slot_rows : Hg;
+                float4* to = reinterpret_cast<float4*>(prefix ? a.o_prefix : a.o_tail) + (size_t)place * (D / 4) * rows_of + mine;
 #pragma unroll 1
                 for (int c = 0; c < D / 32; ++c) {
                     uint32_t o[32];
@@ -250,10 +285,11 @@ attn_shared_tc_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_con
                     tmem_wait_ld();
                     if (mine < rows) {
 #pragma unroll
-                        for (int v4 = 0; v4 < 8; ++v4) reinterpret_cast<uint4*>(orow + c * 32)[v4] = make_uint4(o[4 * v4], o[4 * v4 + 1], o[4 * v4 + 2], o[4 * v4 + 3]);
+                        for (int v4 = 0; v4 < 8; ++v4)
+                            to[(size_t)(c * 8 + v4) * rows_of] = make_float4(__uint_as_float(o[4 * v4]), __uint_as_float(o[4 * v4 + 1]), __uint_as_float(o[4 * v4 + 2]), __uint_as_float(o[4 * v4 + 3]));
                     }
                 }
-                if (mine < rows) (prefix ? a.ml_prefix : a.ml_tail)[row] = make_float2(m_ref, l);
+                if (mine < rows) (prefix ? a.ml_prefix : a.ml_tail)[(size_t)place * rows_of + mine] = make_float2(m_ref, l);
             }
             tc_fence_before();
             mbar_arrive(o_free);
@@ -311,13 +347,13 @@ MI_EXPORT int mi_attn_shared_tc(const void* q, int q_stride, const void* k_cache
            row_tiles_of(H, KV, most), tile_rows_of(H, KV), slot_rows_of(H, KV, most)};
     place_scratch(a, scratch(R, G, H, KV, D, a.row_tiles, a.slot_rows, blocks), work);
     const auto bytes = [&](int ints) { return (size_t)BQ * D * 2 + 4 * (size_t)KT * D * 2 + 16 * 8 + (size_t)ints * 4 + 1024; };
-    const size_t smem = bytes(shared_plan_ints(G, R)), most_smem = bytes(3 * MAX_ENTITIES + 1);
+    const size_t smem = bytes(plan_ints(G, R)), most_smem = bytes(6 * MAX_ENTITIES + 1);
     const float scale_log2 = scale * LOG2E;
 #define LAUNCH(DD) do { \
         cudaError_t e = cudaFuncSetAttribute(attn_shared_tc_kernel<DD>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)most_smem); \
         if (e == cudaSuccess) e = launch_pdl(attn_shared_tc_kernel<DD>, dim3(blocks), dim3(THREADS), smem, stream, kmap, vmap, a, (const __nv_bfloat16*)q, \
                                              (long long)q_stride, scale_log2, error_word); \
-        if (e == cudaSuccess) e = launch_pdl(merge_kernel<__nv_bfloat16, DD, KT>, dim3(R, KV), dim3(128), 0, stream, a, (__nv_bfloat16*)out); \
+        if (e == cudaSuccess) e = launch_pdl(merge_kernel<__nv_bfloat16, DD>, dim3(R, KV), dim3(128 * MERGE_PARTS), 0, stream, a, (__nv_bfloat16*)out); \
         return (int)e; \
     } while (0)
     if (D == 128) LAUNCH(128);

@@ -10,9 +10,10 @@
 // themselves decide, exactly.
 //
 // Two launches.  beam_slice_kernel: a block takes a slice of one row into registers once, and leaves the slice's maximum, its sum of exponentials and
-// its `num` largest logits in order.  The num-th largest of the threads' own maxima is a bound that at least num logits reach; what reaches it (a few
-// more than num) goes to shared memory and every entry counts those before it.  Where more reach it than fit (many equal logits) the block picks num
-// times the next one.  beam_merge_kernel: a block per group joins the slices' sums, and chooses among their candidates the same way.
+// its `num` largest logits in order.  The num / 8-th largest of each warp's 32 threads' maxima, the least of the eight, is a bound that at least num
+// logits reach; what reaches it (a few more than num) goes to shared memory and every entry counts those before it.  Where more reach it than fit (many
+// equal logits) the num-th of those that found room is the next bound: all candidates differ in their order, so each turn has at least CAP - num fewer.  beam_merge_kernel: a block per group joins the slices' sums, and chooses among their sorted lists the
+// same way: a bound from the lists' heads, then a thread per list follows its list down to the bound.
 #include "common.cuh"
 #include <math.h>
 
@@ -20,8 +21,8 @@ using namespace mi;
 
 namespace {
 
-constexpr int NT = 256, CAP = 1024;                 // threads of a block (at least MAX_NUM); candidates that fit in shared memory
-constexpr int MAX_NUM = 128;
+constexpr int NT = 256, CAP = 1024, BASES = 128;                 // threads of a block (at least MAX_NUM); candidates that fit in shared memory
+constexpr int MAX_NUM = 128, WARPS = NT / 32;
 typedef unsigned long long u64;
 
 struct __align__(16) SliceSum { double sum; float top; int count; };
@@ -38,55 +39,98 @@ __device__ __forceinline__ float key_logit(u64 key) {
 }
 __device__ __forceinline__ int key_token(u64 key) { return (int)(0xffffffffu - (uint32_t)key); }
 
-template <typename T> __device__ __forceinline__ T block_max(T v, T* scratch) {
+template <typename T> __device__ __forceinline__ T warp_largest(T v) {
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) { const T w = __shfl_xor_sync(0xffffffffu, v, o); v = w > v ? w : v; }
-    __syncthreads();
-    if ((threadIdx.x & 31) == 0) scratch[threadIdx.x >> 5] = v;
-    __syncthreads();
-    for (int w = 0; w < NT / 32; ++w) v = scratch[w] > v ? scratch[w] : v;
     return v;
 }
-__device__ __forceinline__ double block_sum(double v, double* scratch) {
+// The `turn`-th largest of a warp's values (lowest: below all of them), and the largest
+template <typename T> __device__ __forceinline__ T warp_nth(T mine, int turn, T lowest, T& largest) {
+    T best = largest = warp_largest(mine);
+    for (int k = 1; k < turn; ++k) {                 // once more without the lane that had it
+        const uint32_t who = __ballot_sync(0xffffffffu, mine == best);
+        if ((threadIdx.x & 31) == __ffs(who) - 1) mine = lowest;
+        best = warp_largest(mine);
+    }
+    return best;
+}
+// A bound that at least num (<= NT) of the threads' values reach: the least over the warps of their num / 8-th largest
+__device__ __forceinline__ int turns(int num) { return (num + WARPS - 1) / WARPS; }
+__device__ __forceinline__ double threshold(double mine, int num, double* scratch) {
+    double largest;
+    double best = warp_nth(mine, turns(num), -(double)INFINITY, largest);
+    __syncthreads();
+    if ((threadIdx.x & 31) == 0) scratch[threadIdx.x >> 5] = best;
+    __syncthreads();
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-    __syncthreads();
-    if ((threadIdx.x & 31) == 0) scratch[threadIdx.x >> 5] = v;
-    __syncthreads();
-    v = 0.;
-    for (int w = 0; w < NT / 32; ++w) v += scratch[w];
-    return v;
+    for (int w = 0; w < WARPS; ++w) best = fmin(best, scratch[w]);
+    return best;
 }
 
-// The num-th largest of the threads' values (num <= NT): at least num of what the threads hold reach it
-template <typename T> __device__ __forceinline__ T threshold(T mine, int num, T* all, T* answer) {
-    __syncthreads();
-    all[threadIdx.x] = mine;
-    __syncthreads();
-    int before = 0;
-    for (int i = 0; i < NT; ++i) { const T o = all[i]; before += o > mine || (o == mine && i < threadIdx.x); }
-    if (before == num - 1) *answer = mine;
-    __syncthreads();
-    return *answer;
-}
+// e^(x - m) for logits x <= m, |m| <= 1024, with errors of about 5e-10 of it, as a leading and a small part: 2^t, t = n + j / 32 + r, is 2^n times a table's 2^(j / 32)
+// times a polynomial in r, |r| <= 1/64 (table-driven, after Tang).  m log2(e) is split into a multiple of 2^-12, to which j / 32 is added without
+// rounding, and the rest, so that r is off by 2^-31 or so.  The table is spread over a warp's lanes.
+constexpr float LOG2E_HI = 0x1.715476p+0f, LOG2E_LO = 0x1.4ae0cp-26f;
+__device__ const float2 POWERS[32] = {        // 2^(j / 32) and what its rounding left
+    {1.f, 0.f}, {1.0218971967697144f, -4.81155986e-08f}, {1.0442737340927124f, 4.83347016e-08f}, {1.0671404600143433f, -5.93375198e-08f},
+    {1.0905077457427979f, -1.30775399e-08f}, {1.114386796951294f, -5.43554002e-08f}, {1.1387885808944702f, 5.38622231e-08f}, {1.1637248992919922f, -4.05144149e-08f},
+    {1.1892070770263672f, 3.79763527e-08f}, {1.215247392654419f, -3.26739489e-08f}, {1.2418577671051025f, 4.4968381e-08f}, {1.2690509557724f, 1.41933332e-09f},
+    {1.2968395948410034f, -4.01899953e-08f}, {1.3252366781234741f, -3.49637332e-08f}, {1.3542555570602417f, -1.01233493e-08f}, {1.3839099407196045f, -5.87557736e-08f},
+    {1.4142135381698608f, 2.4203235e-08f}, {1.4451807737350464f, 3.32419994e-08f}, {1.4768261909484863f, -4.50089885e-08f}, {1.5091644525527954f, -2.49593732e-08f},
+    {1.5422108173370361f, 8.07090483e-09f}, {1.5759809017181396f, -5.66102543e-08f}, {1.610490322113037f, 9.83621717e-09f}, {1.6457555294036865f, -5.12497209e-08f},
+    {1.6817928552627563f, -2.47553267e-08f}, {1.7186193466186523f, -4.8496176e-08f}, {1.7562521696090698f, -9.23577037e-09f}, {1.7947090864181519f, -1.14150449e-08f},
+    {1.8340080976486206f, -1.1239278e-08f}, {1.8741676807403564f, -4.66300563e-08f}, {1.9152065515518188f, 9.84532811e-09f}, {1.9571441411972046f, -1.70218044e-08f}};
+struct Exponential {
+    float2 power;                                    // of this lane
+    float m_hi, m_lo, m_32, least;
+    __device__ __forceinline__ Exponential(float m, const float2& power_) : power(power_) {
+        const double y = (double)m * 1.4426950408889634074;
+        m_hi = (float)(rint(y * 4096.) * (1. / 4096.));
+        m_lo = (float)(y - (double)m_hi);
+        m_32 = -32.f * m_hi;
+        least = m - 44.f;                            // e^-44 = 2^-63: logits below it (-inf among them) count as that
+    }
+    // of two logits at once: adds their leading parts to sum and the rest to rest
+    __device__ __forceinline__ void operator()(float x0, float x1, double& sum, float& rest) const {
+        const float2 x = make_float2(fmaxf(x0, least), fmaxf(x1, least)), magic = make_float2(12582912.f, 12582912.f);
+        const float2 z = __fadd2_rn(__ffma2_rn(x, make_float2(32.f * LOG2E_HI, 32.f * LOG2E_HI), make_float2(m_32, m_32)), magic);      // its last bits: 32 t rounded to a whole number
+        const float2 k = __fadd2_rn(z, make_float2(-12582912.f, -12582912.f));
+        const float2 c = __ffma2_rn(k, make_float2(-1.f / 32.f, -1.f / 32.f), make_float2(-m_hi, -m_hi));
+        const float2 r = __fadd2_rn(__ffma2_rn(x, make_float2(LOG2E_LO, LOG2E_LO), __ffma2_rn(x, make_float2(LOG2E_HI, LOG2E_HI), c)), make_float2(-m_lo, -m_lo));
+        float2 p = __ffma2_rn(r, make_float2(0x1.3b2ab6p-7f, 0x1.3b2ab6p-7f), make_float2(0x1.c6b08ep-5f, 0x1.c6b08ep-5f));                // ln(2)^i / i!
+        p = __ffma2_rn(r, p, make_float2(0x1.ebfbep-3f, 0x1.ebfbep-3f));
+        p = __fmul2_rn(r, __ffma2_rn(r, p, make_float2(0x1.62e43p-1f, 0x1.62e43p-1f)));
+        const int k0 = __float_as_int(z.x), k1 = __float_as_int(z.y);      // the magic number's own last bits are 0
+        const float2 hi = make_float2(__shfl_sync(0xffffffffu, power.x, k0), __shfl_sync(0xffffffffu, power.x, k1));
+        const float2 lo = make_float2(__shfl_sync(0xffffffffu, power.y, k0), __shfl_sync(0xffffffffu, power.y, k1));
+        // 2^floor(k / 32): bits 5 and up of k (mod 2^8) into the exponent
+        const float2 scale = make_float2(__int_as_float(((k0 >> 5) + 127) << 23), __int_as_float(((k1 >> 5) + 127) << 23));
+        const float2 lead = __fmul2_rn(hi, scale), small = __fmul2_rn(__ffma2_rn(hi, p, lo), scale);
+        sum += (double)lead.x;
+        sum += (double)lead.y;
+        rest += small.x + small.y;
+    }
+};
 
 // EPT logits a thread, four neighbours at a time
 template <int EPT>
-__global__ void __launch_bounds__(NT) beam_slice_kernel(const float* __restrict__ logits, long long ld, int vocab, int num, SliceSum* __restrict__ sums,
-                                                        u64* __restrict__ keys) {
-    __shared__ union { double d[NT / 32]; float f[NT / 32]; u64 u[NT / 32]; } scratch;
-    __shared__ float maxima[NT], bound;
-    __shared__ u64 found[CAP];
+__global__ void __launch_bounds__(NT, 4) beam_slice_kernel(const float* __restrict__ logits, long long ld, int vocab, int num, SliceSum* __restrict__ sums,
+                                                           u64* __restrict__ keys) {
+    __shared__ float tops[WARPS], bounds[WARPS];
+    __shared__ double parts[WARPS];
+    __shared__ u64 found[CAP], floor_of;
     __shared__ int count;
     pdl_trigger();
+    const float2 power = POWERS[threadIdx.x & 31];
     pdl_wait(logits);
-    const int r = blockIdx.y, slice = blockIdx.x, slices = gridDim.x, base = slice * NT * EPT;
+    const int r = blockIdx.y, slice = blockIdx.x, slices = gridDim.x, base = slice * NT * EPT, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const float* row = logits + (long long)r * ld;
     const bool vec = ((uintptr_t)row & 15) == 0;
+    const auto index = [&](int e) { return base + ((e >> 2) * NT + (int)threadIdx.x) * 4 + (e & 3); };
     float x[EPT];
 #pragma unroll
     for (int k = 0; k < EPT / 4; ++k) {
-        const int i = base + (k * NT + threadIdx.x) * 4;
+        const int i = index(4 * k);
         if (vec && i + 3 < vocab) {
             load16(row + i, x + 4 * k);
         } else {
@@ -99,73 +143,110 @@ __global__ void __launch_bounds__(NT) beam_slice_kernel(const float* __restrict_
 #pragma unroll
     for (int e = 0; e < EPT; ++e) {
         bad |= !(x[e] < INFINITY);
-        x[e] += 0.f;                                 // -0 is 0
         top = fmaxf(top, x[e]);
     }
+    if (bad) top = INFINITY;
+    float largest;
+    const float nth = warp_nth(top, turns(num), -INFINITY, largest);
     if (threadIdx.x == 0) count = 0;
-    const float m = block_max(top, scratch.f);
-    bad = __syncthreads_or(bad);
+    if (lane == 0) { tops[warp] = largest; bounds[warp] = nth; }
+    __syncthreads();
+    float m = tops[0], least = bounds[0];
+#pragma unroll
+    for (int w = 1; w < WARPS; ++w) { m = fmaxf(m, tops[w]); least = fminf(least, bounds[w]); }
     SliceSum* out = sums + (size_t)r * slices + slice;
-    if (bad || m == -INFINITY) {
-        if (threadIdx.x == 0) *out = SliceSum{bad ? (double)NAN : 0., m, 0};
+    u64* best = keys + ((size_t)r * slices + slice) * num;
+    if (!(fabsf(m) < INFINITY)) {                    // NaN or +inf (the row offers nothing), or nothing above -inf
+        if (threadIdx.x == 0) *out = SliceSum{m == -INFINITY ? 0. : (double)NAN, m, 0};
+        for (int k = threadIdx.x; k < num; k += NT) best[k] = 0;
         return;
     }
     double sum = 0.;
+    if (fabsf(m) <= 1024.f) {
+        const Exponential exponential(m, power);
+        float rest = 0.f;
 #pragma unroll
-    for (int e = 0; e < EPT; ++e) sum += exp((double)x[e] - (double)m);
-    sum = block_sum(sum, scratch.d);
-
-    const float least = threshold(top, num, maxima, &bound);
+        for (int e = 0; e < EPT; e += 2) exponential(x[e], x[e + 1], sum, rest);
+        sum += (double)rest;
+    } else {
 #pragma unroll
-    for (int e = 0; e < EPT; ++e)
-        if (x[e] >= least && x[e] > -INFINITY) {
-            const int at = atomicAdd(&count, 1);
-            if (at < CAP) found[at] = logit_key(x[e], base + ((e >> 2) * NT + threadIdx.x) * 4 + (e & 3));
+        for (int e = 0; e < EPT; ++e) sum += exp((double)x[e] - (double)m);
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+    if (lane == 0) parts[warp] = sum;
+    uint32_t hits = 0;                               // few of a thread's logits reach the bound: those are read once more
+#pragma unroll
+    for (int e = 0; e < EPT; ++e) hits |= (x[e] >= least && x[e] > -INFINITY ? 1u : 0u) << e;
+    int n;
+    for (u64 floor_key = 0;;) {
+        for (uint32_t left = hits; left; left &= left - 1) {
+            const int i = index(__ffs(left) - 1);
+            const u64 key = logit_key(row[i] + 0.f, i);      // -0 is 0
+            if (key >= floor_key) {
+                const int at = atomicAdd(&count, 1);
+                if (at < CAP) found[at] = key;
+            }
         }
-    __syncthreads();
-    const int n = count;
-    u64* best = keys + ((size_t)r * slices + slice) * num;
-    if (n <= CAP) {
-        for (int i = threadIdx.x; i < n; i += NT) {
+        __syncthreads();
+        n = count;
+        if (n <= CAP) break;
+        for (int i = threadIdx.x; i < CAP; i += NT) {
             const u64 mine = found[i];
             int before = 0;
-            for (int o = 0; o < n; ++o) before += found[o] > mine;
-            if (before < num) best[before] = mine;
+            for (int o = 0; o < CAP; ++o) before += found[o] > mine;
+            if (before == num - 1) floor_of = mine;
         }
-    } else {
-        u64 last = ~0ull;
-        for (int k = 0; k < num; ++k) {
-            u64 next = 0;
-#pragma unroll
-            for (int e = 0; e < EPT; ++e) {
-                const u64 key = x[e] > -INFINITY ? logit_key(x[e], base + ((e >> 2) * NT + threadIdx.x) * 4 + (e & 3)) : 0;
-                if (key < last && key > next) next = key;
-            }
-            last = block_max(next, scratch.u);
-            if (threadIdx.x == 0) best[k] = last;
-        }
+        __syncthreads();
+        floor_key = floor_of;
+        if (threadIdx.x == 0) count = 0;
+        __syncthreads();
     }
-    if (threadIdx.x == 0) *out = SliceSum{sum, m, min(n, num)};
+    for (int i = threadIdx.x; i < n; i += NT) {
+        const u64 mine = found[i];
+        int before = 0;
+#pragma unroll 8
+        for (int o = 0; o < n; ++o) before += found[o] > mine;
+        if (before < num) best[before] = mine;
+    }
+    for (int k = n + threadIdx.x; k < num; k += NT) best[k] = 0;
+    if (threadIdx.x == 0) {
+        for (int w = 1; w < WARPS; ++w) sum += parts[w];
+        *out = SliceSum{sum, m, min(n, num)};
+    }
 }
 
 struct Candidate { double value; int row; u64 key; };
 __device__ __forceinline__ bool goes_before(const Candidate& a, const Candidate& b) {
     return a.value != b.value ? a.value > b.value : a.row != b.row ? a.row < b.row : a.key > b.key;
 }
+struct Found {                                       // candidates in shared memory
+    double value[CAP]; u64 key[CAP]; int row[CAP];
+    __device__ __forceinline__ Candidate get(int i) const { return Candidate{value[i], row[i], key[i]}; }
+    __device__ __forceinline__ void put(int i, const Candidate& c) { value[i] = c.value; key[i] = c.key; row[i] = c.row; }
+    __device__ __forceinline__ int before(const Candidate& c, int n) const {       // how many of the first n go before c, which is one of them
+        int before = 0, same = 0;
+#pragma unroll 8
+        for (int o = 0; o < n; ++o) { const double v = value[o]; before += v > c.value; same += v == c.value; }
+        if (same > 1)
+            for (int o = 0; o < n; ++o) before += value[o] == c.value && (row[o] != c.row ? row[o] < c.row : key[o] > c.key);
+        return before;
+    }
+};
 
 __global__ void __launch_bounds__(NT) beam_merge_kernel(const SliceSum* sums, const u64* keys, int slices, int num, const float* __restrict__ scores, int rows,
                                                         const int* __restrict__ group_start, double* base, float* __restrict__ values, int* __restrict__ out_rows,
                                                         int* __restrict__ out_tokens) {
-    __shared__ double maxima[NT], bound;
-    __shared__ Candidate found[CAP];
-    __shared__ Candidate warp_best[NT / 32];
+    __shared__ double scratch[WARPS], near_base[BASES];
+    __shared__ Found found;
+    __shared__ Candidate bound;
     __shared__ int count;
     pdl_trigger();
     pdl_wait(scores, group_start);
     const int g = blockIdx.x, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int a = max(0, min(group_start[g], rows)), b = max(a, min(group_start[g + 1], rows));
     // s[r] - lse[r], a warp per row
-    for (int r = a + warp; r < b; r += NT / 32) {
+    for (int r = a + warp; r < b; r += WARPS) {
         const SliceSum* mine = sums + (size_t)r * slices;
         float m = -INFINITY;
         for (int i = lane; i < slices; i += 32) m = fmaxf(m, mine[i].top);
@@ -175,65 +256,89 @@ __global__ void __launch_bounds__(NT) beam_merge_kernel(const SliceSum* sums, co
 #pragma unroll
         for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
         const double v = (double)scores[r] - ((double)m + log(sum));
-        if (lane == 0) base[r] = isfinite(v) ? v : -(double)INFINITY;
+        if (lane == 0) { base[r] = isfinite(v) ? v : -(double)INFINITY; if (r - a < BASES) near_base[r - a] = base[r]; }
     }
     if (threadIdx.x == 0) count = 0;
     __syncthreads();
-    // candidate i: row, slice, place in the slice's list
-    const long long n = (long long)(b - a) * slices * num;
-    auto at = [&](long long i) {
-        const int list = (int)(i / num), k = (int)(i % num), r = a + list / slices;
+    // list i: row, slice; candidate k of it
+    const int lists = (b - a) * slices;
+    const auto at = [&](int list, int k) {
+        const int r = a + list / slices;
         const size_t where = (size_t)r * slices + list % slices;
         Candidate c{-(double)INFINITY, r, 0};
-        const double from = base[r];
-        if (k < sums[where].count && from != -(double)INFINITY) {
-            c.key = keys[where * num + k];
-            c.value = from + (double)key_logit(c.key);
-        }
+        const double from = r - a < BASES ? near_base[r - a] : base[r];
+        if (k < num) c.key = keys[where * num + k];
+        if (c.key) c.value = from + (double)key_logit(c.key);
         return c;
     };
-    double top = -(double)INFINITY;
-    for (long long i = threadIdx.x; i < n; i += NT) top = fmax(top, at(i).value);
-    const double least = threshold(top, num, maxima, &bound);
-    for (long long i = threadIdx.x; i < n; i += NT) {
-        const Candidate c = at(i);
-        if (c.value >= least && c.value > -(double)INFINITY) {
-            const int p = atomicAdd(&count, 1);
-            if (p < CAP) found[p] = c;
-        }
-    }
-    __syncthreads();
-    const int have = count;
-    auto write = [&](int place, const Candidate& c) {
-        const size_t o = (size_t)g * num + place;
-        values[o] = (float)c.value; out_rows[o] = c.row; out_tokens[o] = key_token(c.key);
-    };
-    if (have <= CAP) {
-        for (int i = threadIdx.x; i < have; i += NT) {
-            const Candidate mine = found[i];
-            int before = 0;
-            for (int o = 0; o < have; ++o) before += goes_before(found[o], mine);
-            if (before < num) write(before, mine);
-        }
+    // A value that at least num candidates reach: from the heads where every warp has enough lists (list i belongs to warp i % 8), else the least of
+    // the depth-th candidates, depth the number of lists in num.
+    const int first = lane * WARPS + warp;
+    double least;
+    if (lists / WARPS >= turns(num)) {
+        double top = -(double)INFINITY;
+        for (int i = first; i < lists; i += NT) top = fmax(top, at(i, 0).value);
+        least = threshold(top, num, scratch);
     } else {
-        Candidate last{(double)INFINITY, -1, 0};
-        for (int k = 0; k < num; ++k) {              // the first of those behind the last one
-            Candidate next{-(double)INFINITY, 0x7fffffff, 0};
-            for (long long i = threadIdx.x; i < n; i += NT) {
-                const Candidate c = at(i);
-                if (c.value >= least && c.value > -(double)INFINITY && goes_before(last, c) && goes_before(c, next)) next = c;
+        const int depth = lists ? (num + lists - 1) / lists : 1;
+        double low = (double)INFINITY;
+        for (int i = first; i < lists; i += NT) low = fmin(low, at(i, depth - 1).value);
+        low = -warp_largest(-low);
+        if (lane == 0) scratch[warp] = low;
+        __syncthreads();
+        least = scratch[0];
+        for (int w = 1; w < WARPS; ++w) least = fmin(least, scratch[w]);
+    }
+    int have;
+    for (bool bounded = false;; bounded = true) {
+        for (int i = first; i < lists; i += NT)
+            for (int k = 0; k < num; ++k) {
+                const Candidate c = at(i, k);
+                if (!(c.value >= least && c.value > -(double)INFINITY) || (bounded && goes_before(bound, c))) break;      // lists are in order
+                const int p = atomicAdd(&count, 1);
+                if (p < CAP) found.put(p, c);
             }
+        __syncthreads();
+        have = count;
+        if (have <= CAP) break;
+        for (int i = threadIdx.x; i < CAP; i += NT) {
+            const Candidate mine = found.get(i);
+            if (found.before(mine, CAP) == num - 1) bound = mine;
+        }
+        __syncthreads();
+        if (threadIdx.x == 0) count = 0;
+        __syncthreads();
+    }
+    // many more than num reach the bound: a better one, from the candidates themselves, while it leaves a good part of them out
+    while (have > num + NT / 4) {
+        constexpr int MINE = CAP / NT;
+        Candidate mine[MINE];
+        double top = -(double)INFINITY;
 #pragma unroll
-            for (int o = 16; o > 0; o >>= 1) {
-                const Candidate w{__shfl_xor_sync(0xffffffffu, next.value, o), __shfl_xor_sync(0xffffffffu, next.row, o), __shfl_xor_sync(0xffffffffu, next.key, o)};
-                if (goes_before(w, next)) next = w;
-            }
-            __syncthreads();
-            if (lane == 0) warp_best[warp] = next;
-            __syncthreads();
-            last = warp_best[0];
-            for (int w = 1; w < NT / 32; ++w) if (goes_before(warp_best[w], last)) last = warp_best[w];
-            if (threadIdx.x == 0) write(k, last);
+        for (int e = 0; e < MINE; ++e) {
+            const int i = threadIdx.x + e * NT;
+            mine[e] = i < have ? found.get(i) : Candidate{-(double)INFINITY, 0, 0};
+            top = fmax(top, mine[e].value);
+        }
+        least = threshold(top, num, scratch);      // (its barriers stand between the reads and the writes)
+        if (threadIdx.x == 0) count = 0;
+        __syncthreads();
+#pragma unroll
+        for (int e = 0; e < MINE; ++e)
+            if (mine[e].value >= least && mine[e].value > -(double)INFINITY) found.put(atomicAdd(&count, 1), mine[e]);
+        __syncthreads();
+        const int left = count;
+        const bool enough = left > have - have / 4;
+        have = left;
+        __syncthreads();
+        if (enough) break;
+    }
+    for (int i = threadIdx.x; i < have; i += NT) {
+        const Candidate mine = found.get(i);
+        const int before = found.before(mine, have);
+        if (before < num) {
+            const size_t o = (size_t)g * num + before;
+            values[o] = (float)mine.value; out_rows[o] = mine.row; out_tokens[o] = key_token(mine.key);
         }
     }
     for (int k = have + threadIdx.x; k < num; k += NT) {
@@ -244,9 +349,7 @@ __global__ void __launch_bounds__(NT) beam_merge_kernel(const SliceSum* sums, co
 
 int slice_size(int rows, int vocab) {
     // enough blocks for two an SM where the logits allow it
-    for (int ept : {32, 16})
-        if ((long long)rows * ((vocab + NT * ept - 1) / (NT * ept)) >= 2ll * device_sms()) return ept;
-    return 8;
+    return (long long)rows * ((vocab + NT * 16 - 1) / (NT * 16)) >= 2ll * device_sms() ? 16 : 8;
 }
 
 }  // namespace
@@ -272,8 +375,7 @@ MI_EXPORT int mi_beam_select(const float* logits, long long ld, int rows, int vo
     if (rows) {
         cudaError_t e;
         const dim3 grid(slices, rows);
-        if (ept == 32) e = launch_pdl(beam_slice_kernel<32>, grid, dim3(NT), 0, stream, logits, ld, vocab, num, sums, keys);
-        else if (ept == 16) e = launch_pdl(beam_slice_kernel<16>, grid, dim3(NT), 0, stream, logits, ld, vocab, num, sums, keys);
+        if (ept == 16) e = launch_pdl(beam_slice_kernel<16>, grid, dim3(NT), 0, stream, logits, ld, vocab, num, sums, keys);
         else e = launch_pdl(beam_slice_kernel<8>, grid, dim3(NT), 0, stream, logits, ld, vocab, num, sums, keys);
         if (e != cudaSuccess) return (int)e;
     }

@@ -9,6 +9,7 @@ of float32 sums whether they run as multiply-adds or as bfloat16 parts on the te
 """
 from __future__ import annotations
 
+import array
 import contextlib
 import ctypes
 import math
@@ -65,6 +66,7 @@ def load_calls():
 
 
 _CODES = {torch.float32: 0, torch.bfloat16: 1}
+_NOTHING = contextlib.nullcontext()
 
 
 def _code(dtype):
@@ -617,9 +619,11 @@ class CudaOps:
             self.launches += 1
         if not num_decode:
             return out
-        if not win and not split_weights and getattr(meta, "shared_start", None) is not None and self._takes_shared(q, k_cache, v_cache, meta, H, KV, D):
-            self._shared_decode(q, k_cache, v_cache, out, meta, H, KV, D, scale)
-            return out
+        if not win and not split_weights and getattr(meta, "shared_start", None) is not None:
+            size = self._shared_bytes(q, k_cache, v_cache, meta, H, KV, D)
+            if size > 0:
+                self._shared_decode(q, k_cache, v_cache, out, meta, H, KV, D, scale, size)
+                return out
         fast_decode = fast and H // KV <= 16 and meta.page_size % 16 == 0
         S = self.choose_splits(num_decode * (KV if fast_decode else math.ceil(H / 4)), meta.max_kv_len,
                                (2 if self.bulk_decode else 3) if fast_decode else 2,
@@ -665,49 +669,67 @@ class CudaOps:
         without keys gets zeros.  The output [T, H D] has the entries' rows; others are left as they come.
         Heads of 64 or 128 run on kernels that share; other heads, more than 4,096 entries and groups, and bfloat16 pages that neither divide 64 keys
         nor are divided by them are computed row by row, by the rows' own pages."""
-        if q.dim() != 2 or q.shape[1] != H * D or H < 1 or KV < 1 or H % KV or (q.shape[1] > 1 and q.stride(1) != 1):
-            raise ValueError(f"shared_prefix_attention: queries {tuple(q.shape)} with strides {q.stride()} are no rows of {H} heads of {D} over {KV} key heads")
-        if k_cache.shape != v_cache.shape or k_cache.dim() != 4 or tuple(k_cache.shape[1:]) != (KV, meta.page_size, D):
-            raise ValueError(f"shared_prefix_attention: caches {tuple(k_cache.shape)} and {tuple(v_cache.shape)} are not [pages, {KV}, {meta.page_size}, {D}]")
-        if not scale > 0:
-            raise ValueError(f"shared_prefix_attention: scale {scale} is not positive")
+        rows = getattr(meta, "table_rows", None)
+        lists = (meta.decode_segs, meta.seg_q_start, meta.seg_kv_len, meta.shared_start, meta.shared_len)
+        tables = (meta.block_table,) if rows is None else (meta.block_table, rows)
+        dtype, here = q.dtype, self._device_index
+        for t in lists + tables:                         # one quick look; what is wrong is found out where something is
+            if t.dtype is not torch.int32 or not t.is_contiguous() or t.get_device() != here:
+                break
+        else:
+            if (len(q.shape) == 2 and q.shape[1] == H * D and H > 0 and KV > 0 and H % KV == 0 and q.stride(1) == 1 and scale > 0 and dtype in _CODES
+                    and k_cache.dtype is dtype and v_cache.dtype is dtype and k_cache.is_contiguous() and v_cache.is_contiguous()
+                    and k_cache.shape == v_cache.shape and k_cache.shape[1:] == (KV, meta.page_size, D) and meta.block_table.shape[1:] == (meta.max_pages,)
+                    and lists[0].dim() == lists[1].dim() == lists[2].dim() == lists[3].dim() == lists[4].dim() == 1 and lists[3].shape[0] == lists[4].shape[0] + 1
+                    and q.get_device() == k_cache.get_device() == v_cache.get_device() == here):
+                return self._shared_or_alone(q, k_cache, v_cache, meta, H, KV, D, scale)
+        self._refuse_shared(q, k_cache, v_cache, meta, H, KV, D, scale, lists, tables)
+
+    def _refuse_shared(self, q, k_cache, v_cache, meta, H, KV, D, scale, lists, tables):
+        """Raises what is wrong with a call of shared_prefix_attention."""
+        what = "shared_prefix_attention"
+        named = dict(zip(("decode_segs", "seg_q_start", "seg_kv_len", "shared_start", "shared_len"), lists)) | dict(zip(("block_table", "table_rows"), tables))
+        if q.dim() != 2 or H < 1 or KV < 1 or H % KV or q.shape[1] != H * D or q.stride(1) != 1:
+            raise ValueError(f"{what}: queries {tuple(q.shape)} with strides {q.stride()} are no rows of {H} heads of {D} over {KV} key heads")
         if _code(q.dtype) != _code(k_cache.dtype) or k_cache.dtype != v_cache.dtype:
-            raise TypeError(f"shared_prefix_attention: queries {q.dtype}, caches {k_cache.dtype} and {v_cache.dtype}")
-        lists = dict(decode_segs=meta.decode_segs, seg_q_start=meta.seg_q_start, seg_kv_len=meta.seg_kv_len, shared_start=meta.shared_start, shared_len=meta.shared_len)
-        if getattr(meta, "table_rows", None) is not None:
-            lists["table_rows"] = meta.table_rows
-        self._plain("shared_prefix_attention", torch.int32, block_table=meta.block_table, **lists)
-        self._plain("shared_prefix_attention", k_cache.dtype, k_cache=k_cache, v_cache=v_cache)
-        if any(t.dim() != 1 for t in lists.values()) or meta.shared_start.shape[0] != meta.shared_len.shape[0] + 1:
-            raise ValueError(f"shared_prefix_attention: shared_start {tuple(meta.shared_start.shape)} and shared_len {tuple(meta.shared_len.shape)} do not fit together")
+            raise TypeError(f"{what}: queries {q.dtype}, caches {k_cache.dtype} and {v_cache.dtype}")
+        if k_cache.shape != v_cache.shape or k_cache.dim() != 4 or tuple(k_cache.shape[1:]) != (KV, meta.page_size, D):
+            raise ValueError(f"{what}: caches {tuple(k_cache.shape)} and {tuple(v_cache.shape)} are not [pages, {KV}, {meta.page_size}, {D}]")
+        if not scale > 0:
+            raise ValueError(f"{what}: scale {scale} is not positive")
+        self._plain(what, torch.int32, **named)
+        self._plain(what, k_cache.dtype, k_cache=k_cache, v_cache=v_cache)
+        if any(t.dim() != 1 for t in lists) or meta.shared_start.shape[0] != meta.shared_len.shape[0] + 1:
+            raise ValueError(f"{what}: the lists have shapes { {k: tuple(t.shape) for k, t in named.items()} }")
         if meta.block_table.dim() != 2 or meta.block_table.shape[1] != meta.max_pages:
-            raise ValueError(f"shared_prefix_attention: block_table {tuple(meta.block_table.shape)} has no {meta.max_pages} pages a row")
-        self._here("shared_prefix_attention", q=q, k_cache=k_cache, v_cache=v_cache, block_table=meta.block_table, **lists)
+            raise ValueError(f"{what}: block_table {tuple(meta.block_table.shape)} has no {meta.max_pages} pages a row")
+        self._here(what, q=q, k_cache=k_cache, v_cache=v_cache, **named)
+        raise AssertionError(f"{what}: refused without a reason")
+
+    def _shared_or_alone(self, q, k_cache, v_cache, meta, H, KV, D, scale):
         with self._current():
-            if not self._takes_shared(q, k_cache, v_cache, meta, H, KV, D):
+            size = self._shared_bytes(q, k_cache, v_cache, meta, H, KV, D)
+            if size <= 0:
                 alone = types.SimpleNamespace(prefill_tiles=meta.decode_segs[:0].view(0, 2), tile=self.prefill_tile, max_kv_len=meta.max_kv_len, max_pages=meta.max_pages,
                                               page_size=meta.page_size, block_table=meta.block_table, table_rows=getattr(meta, "table_rows", None), shared_start=None,
-                                              **{k: lists[k] for k in ("decode_segs", "seg_q_start", "seg_kv_len")})
+                                              decode_segs=meta.decode_segs, seg_q_start=meta.seg_q_start, seg_kv_len=meta.seg_kv_len)
                 return self.paged_attention(q, k_cache, v_cache, alone, H, KV, D, scale, None)
-            out = torch.empty((q.shape[0], H * D), dtype=q.dtype, device=q.device)
-            self._shared_decode(q, k_cache, v_cache, out, meta, H, KV, D, scale)
+            out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+            self._shared_decode(q, k_cache, v_cache, out, meta, H, KV, D, scale, size)
         return out
 
-    def _takes_shared(self, q, k_cache, v_cache, meta, H, KV, D):
-        """Whether a kernel that reads shared prefixes once takes these rows."""
+    def _shared_bytes(self, q, k_cache, v_cache, meta, H, KV, D):
+        """Bytes of scratch of the kernel that reads shared prefixes once; not above 0: these rows are computed one by one."""
         if not self.fast_attention or q.stride(0) % (16 // q.element_size()) or (q.data_ptr() | k_cache.data_ptr() | v_cache.data_ptr()) % 16:
-            return False
-        return self._shared_bytes(q, meta, H, KV, D) > 0
+            return 0
+        size = self.lib.mi_attn_shared_tc_bytes if q.dtype is torch.bfloat16 else self.lib.mi_attn_shared_f32_bytes
+        return size(meta.decode_segs.shape[0], meta.shared_len.shape[0], meta.max_shared_rows, H, KV, D, meta.page_size)
 
-    def _shared_bytes(self, q, meta, H, KV, D):
-        size = self.lib.mi_attn_shared_tc_bytes if q.dtype == torch.bfloat16 else self.lib.mi_attn_shared_f32_bytes
-        return int(size(meta.decode_segs.shape[0], meta.shared_len.shape[0], meta.max_shared_rows, H, KV, D, meta.page_size))
-
-    def _shared_decode(self, q, k_cache, v_cache, out, meta, H, KV, D, scale):
-        work = torch.empty(self._shared_bytes(q, meta, H, KV, D), dtype=torch.uint8, device=q.device)
+    def _shared_decode(self, q, k_cache, v_cache, out, meta, H, KV, D, scale, size):
+        work = torch.empty(size, dtype=torch.uint8, device=q.device)
         rows = (out, meta.decode_segs, meta.decode_segs.shape[0], meta.seg_q_start, meta.seg_kv_len, meta.block_table, getattr(meta, "table_rows", None), meta.max_pages,
                 meta.shared_start, meta.shared_len, meta.shared_len.shape[0], meta.max_shared_rows, H, KV, D, meta.page_size, scale, work)
-        if q.dtype == torch.bfloat16:
+        if q.dtype is torch.bfloat16:
             _check(self.lib.mi_attn_shared_tc(q, q.stride(0), k_cache, v_cache, k_cache.shape[0] * KV * meta.page_size, *rows, self._stream_error, self._stream()),
                    "attn_shared_tc")
         else:
@@ -1780,7 +1802,7 @@ class CudaOps:
 
     def _current(self):
         """The device made current for a launch, where another one is."""
-        return contextlib.nullcontext() if torch.cuda.current_device() == self._device_index else torch.cuda.device(self._device_index)
+        return _NOTHING if torch.cuda.current_device() == self._device_index else torch.cuda.device(self._device_index)
 
     def beam_select(self, logits, scores, group_start, num):
         """A beam search step's candidates.  logits float32 [R, V] (rows may be strided), scores float32 [R]: a row per beam and the sum of
@@ -1789,30 +1811,37 @@ class CudaOps:
         (num at most 128): the best of each group, best first; equal values: the lower row, then the larger logit, then the lower token.  Values are
         compared in float64.  Tokens with a logit of -inf are no candidates, nor are rows whose logits hold NaN or +inf or nothing finite or whose
         score is not finite; places that stay empty hold (-inf, -1, -1)."""
-        self._plain("beam_select", torch.float32, scores=scores)
-        self._plain("beam_select", torch.int32, group_start=group_start)
-        if logits.dtype != torch.float32:
-            raise TypeError(f"beam_select: logits are {logits.dtype}, expected torch.float32")
-        if logits.dim() != 2 or scores.dim() != 1 or scores.shape[0] != logits.shape[0] or group_start.dim() != 1 or group_start.shape[0] < 1:
-            raise ValueError(f"beam_select: logits {tuple(logits.shape)}, scores {tuple(scores.shape)} and group_start {tuple(group_start.shape)} do not fit together")
-        (R, V), G = logits.shape, group_start.shape[0] - 1
-        if not 1 <= num <= self.MAX_CANDIDATES:
-            raise ValueError(f"beam_select: {num} candidates a group, between 1 and {self.MAX_CANDIDATES} are possible")
-        if V < 1 or (V > 1 and logits.stride(1) != 1) or (R > 1 and logits.stride(0) < V):
+        here = self._device_index
+        if (logits.dtype is not torch.float32 or scores.dtype is not torch.float32 or group_start.dtype is not torch.int32 or len(logits.shape) != 2 or scores.dim() != 1
+                or group_start.dim() != 1 or not scores.is_contiguous() or not group_start.is_contiguous() or scores.shape[0] != logits.shape[0]
+                or group_start.shape[0] < 1 or not 1 <= num <= self.MAX_CANDIDATES or not logits.get_device() == scores.get_device() == group_start.get_device() == here):
+            self._refuse_select(logits, scores, group_start, num)
+        (R, V), G, ld = logits.shape, group_start.shape[0] - 1, logits.stride(0)
+        if V < 1 or (V > 1 and logits.stride(1) != 1) or (R > 1 and ld < V):
             raise ValueError(f"beam_select: logits of shape {tuple(logits.shape)} with strides {logits.stride()} (a row's logits lie side by side)")
-        self._here("beam_select", logits=logits, scores=scores, group_start=group_start)
         dev = logits.device
         values = torch.empty((G, num), dtype=torch.float32, device=dev)
         rows, tokens = torch.empty((G, num), dtype=torch.int32, device=dev), torch.empty((G, num), dtype=torch.int32, device=dev)
         with self._current():
-            n = int(self.lib.mi_beam_select_bytes(R, V, num))
+            n = self.lib.mi_beam_select_bytes(R, V, num)
             if n < 0:
                 _check(n, "beam_select")
-            work = torch.empty(max(n, 16), dtype=torch.uint8, device=dev)
-            _check(self.lib.mi_beam_select(logits, logits.stride(0) if R > 1 else V, R, V, scores, group_start, G, num, values, rows, tokens, work, self._stream()),
-                   "beam_select")
+            work = torch.empty(n, dtype=torch.uint8, device=dev)
+            _check(self.lib.mi_beam_select(logits, ld if R > 1 else V, R, V, scores, group_start, G, num, values, rows, tokens, work, self._stream()), "beam_select")
         self.launches += (2 if R else 1) if G else 0
         return values, rows, tokens
+
+    def _refuse_select(self, logits, scores, group_start, num):
+        """Raises what is wrong with a call of beam_select."""
+        if logits.dtype != torch.float32:
+            raise TypeError(f"beam_select: logits are {logits.dtype}, expected torch.float32")
+        self._plain("beam_select", torch.float32, scores=scores)
+        self._plain("beam_select", torch.int32, group_start=group_start)
+        if logits.dim() != 2 or scores.dim() != 1 or scores.shape[0] != logits.shape[0] or group_start.dim() != 1 or group_start.shape[0] < 1:
+            raise ValueError(f"beam_select: logits {tuple(logits.shape)}, scores {tuple(scores.shape)} and group_start {tuple(group_start.shape)} do not fit together")
+        if not 1 <= num <= self.MAX_CANDIDATES:
+            raise ValueError(f"beam_select: {num} candidates a group, between 1 and {self.MAX_CANDIDATES} are possible")
+        self._here("beam_select", logits=logits, scores=scores, group_start=group_start)
 
     def reorder_rows(self, tensors, rows, parents, group_start, most, dim=0):
         """In place, for every tensor t of `tensors` and every i: t[rows[i]] = what t[rows[parents[i]]] was before the call (a beam takes over its parent's
@@ -1820,27 +1849,32 @@ class CudaOps:
         from the rows' dimension on, and before it too).  rows, parents int32 [n]; group_start int32 [G + 1]: places group_start[g] .. group_start[g + 1] - 1 of
         both lists are a group, parents (places in the lists) lie in their row's group; most: rows of the largest group, at most 100.  A row is named once.
         A parent outside its group, or a row that a tensor does not have, leaves the row as it is."""
-        tensors = list(tensors)
-        self._plain("reorder_rows", torch.int32, rows=rows, parents=parents, group_start=group_start)
-        if rows.dim() != 1 or rows.shape != parents.shape or group_start.dim() != 1 or group_start.shape[0] < 1:
+        tensors, here = list(tensors), self._device_index
+        if (not (rows.dtype is parents.dtype is group_start.dtype is torch.int32) or not (rows.is_contiguous() and parents.is_contiguous() and group_start.is_contiguous())
+                or rows.dim() != 1 or rows.shape != parents.shape or group_start.dim() != 1 or group_start.shape[0] < 1 or not 0 <= most <= self.MAX_BEAMS):
+            self._plain("reorder_rows", torch.int32, rows=rows, parents=parents, group_start=group_start)
+            if not 0 <= most <= self.MAX_BEAMS:
+                raise ValueError(f"reorder_rows: groups of up to {most} rows, at most {self.MAX_BEAMS} are possible")
             raise ValueError(f"reorder_rows: rows {tuple(rows.shape)}, parents {tuple(parents.shape)} and group_start {tuple(group_start.shape)} do not fit together")
-        if not 0 <= most <= self.MAX_BEAMS:
-            raise ValueError(f"reorder_rows: groups of up to {most} rows, at most {self.MAX_BEAMS} are possible")
-        places = []
+        places = array.array("q")                    # per tensor: address, tables in it, bytes from table to table, rows, bytes from row to row, bytes of a row
         for t in tensors:
-            if not 0 <= dim < t.dim():
-                raise ValueError(f"reorder_rows: a tensor of shape {tuple(t.shape)} has no dimension {dim}")
-            size, n = t.element_size(), t.shape[dim]
-            row = math.prod(t.shape[dim + 1:])
-            stride = t.stride(dim) if n > 1 else row
-            if not t.is_contiguous() and (dim or not t[:1].is_contiguous() or stride < row):
-                raise ValueError(f"reorder_rows: a tensor of shape {tuple(t.shape)} has strides {t.stride()} (rows lie in one piece)")
-            places += (t.data_ptr(), math.prod(t.shape[:dim]), n * stride * size, n, stride * size, row * size)
-        self._here("reorder_rows", rows=rows, parents=parents, group_start=group_start, **{f"tensor {i}": t for i, t in enumerate(tensors)})
-        if places:
-            table = torch.tensor(places, dtype=torch.int64)
+            shape = t.shape
+            if not 0 <= dim < len(shape):
+                raise ValueError(f"reorder_rows: a tensor of shape {tuple(shape)} has no dimension {dim}")
+            size, n = t.element_size(), shape[dim]
+            if t.is_contiguous():
+                lead = math.prod(shape[:dim])
+                row = stride = t.numel() // max(lead * n, 1) * size if n else 0
+            else:
+                lead, row, stride = 1, math.prod(shape[1:]) * size, t.stride(0) * size
+                if dim or not t[:1].is_contiguous() or stride < row:
+                    raise ValueError(f"reorder_rows: a tensor of shape {tuple(shape)} has strides {t.stride()} (rows lie in one piece)")
+            places.extend((t.data_ptr(), lead, n * stride, n, stride, row))
+        if not rows.get_device() == parents.get_device() == group_start.get_device() == here or any(t.get_device() != here for t in tensors):
+            self._here("reorder_rows", rows=rows, parents=parents, group_start=group_start, **{f"tensor {i}": t for i, t in enumerate(tensors)})
+        if tensors:
             with self._current():
-                done = self.lib.mi_reorder_rows(table, len(tensors), rows, parents, group_start, group_start.shape[0] - 1, rows.shape[0], int(most), self._stream())
+                done = self.lib.mi_reorder_rows(places.buffer_info()[0], len(tensors), rows, parents, group_start, group_start.shape[0] - 1, rows.shape[0], most, self._stream())
             if done < 0:
                 _check(done if done > -1000 else -1000 - done, "reorder_rows")
             self.launches += done

@@ -114,7 +114,7 @@ SHAPES = [(32, 8, 128, 16, BF16), (40, 8, 128, 16, BF16), (6, 2, 64, 32, BF16), 
 @pytest.mark.parametrize("name", GROUPS)
 def test_shared_prefix_attention(ops, name, H, KV, D, ps, dtype):
     q, k, v, meta = problem(GROUPS[name], H, KV, D, ps, dtype, seed=len(name) + D)
-    if (name == "no keys" and not ops._takes_shared(q, k, v, meta, H, KV, D)):
+    if (name == "no keys" and ops._shared_bytes(q, k, v, meta, H, KV, D) <= 0):
         pytest.skip("entries without keys: the kernels that share")
     check(ops, q, k, v, meta, H, KV, D)
 
@@ -233,7 +233,7 @@ def test_as_many_entries_as_it_takes(ops):
     for n in (475, 900):                                          # (without garbage where rows are computed alone: that kernel multiplies it by zero)
         takes = 5 * n <= 4096
         q, k, v, meta = problem([(16, [17, 18, 19, 20])] * n, 4, 1, 64, 16, BF16, seed=12, garbage=math.nan if takes else 0.0)
-        assert ops._takes_shared(q, k, v, meta, 4, 1, 64) == takes
+        assert (ops._shared_bytes(q, k, v, meta, 4, 1, 64) > 0) == takes
         check(ops, q, k, v, meta, 4, 1, 64)
 
 
