@@ -7,7 +7,8 @@
 __version__ = "0.1.0"
 
 from .config.engine_args import EngineArgs  # noqa: E402
+from .engine.beam import Beam, BeamParams  # noqa: E402
 from .engine.llm import LLM, create_engine  # noqa: E402
 from .engine.request import SamplingParams  # noqa: E402
 
-__all__ = ["LLM", "SamplingParams", "EngineArgs", "create_engine"]
+__all__ = ["LLM", "SamplingParams", "BeamParams", "Beam", "EngineArgs", "create_engine"]

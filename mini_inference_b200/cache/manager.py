@@ -9,10 +9,15 @@ before the window of the next position (the pages of the first keep_first keys s
 [steps, planes (k, v; or one), pages + 1, kv_heads, page_size, head_dim]: one (page, kv head) is a
 contiguous page_size x head_dim tile that a kernel can fetch in one bulk copy.
 
-Call order for a request: admit -> (ensure -> commit)* -> free.
+Call order for a request: admit -> (ensure -> commit)* -> free.  Beams of a request: admit -> ... -> fork -> (reorder -> ensure -> commit)* -> free of each.
   ensure(seq, n)  pages for positions < n exist in every group, all or nothing
                   (the reference's reserve() keeps a partial grab, kv_cache.py:216-224)
   commit(seq, n)  n tokens are now cached; pages a window has passed are given back
+  fork(seq, ids)  more holds on what seq has cached: its full pages are shared (PagePool.share), the last, partly
+                  filled page and the states are rows of their own that reorder fills
+  reorder(...)    every beam takes over its parent's cache: full pages by reference, the last page and the states by a
+                  copy on the device (in place, all beams of all prompts at once)
+A page that more than one request holds is full, so nobody writes to it.
 
 Block tables live twice: a host array per group ([slots + 1, max pages], the truth) and a
 device copy of the same shape that the attention kernels read, a request's row being its
@@ -24,6 +29,7 @@ new page and a released page per request, whatever the context length.
 from __future__ import annotations
 
 import math
+from collections import Counter
 from typing import List, Optional
 
 import numpy as np
@@ -36,7 +42,7 @@ from .state_slots import StateSlots
 
 class SeqCache:
     """One live request's hold on the cache."""
-    __slots__ = ("seq_id", "slot", "num_tokens", "num_pages", "first_live", "alive")
+    __slots__ = ("seq_id", "slot", "num_tokens", "num_pages", "first_live", "alive", "family")
 
     def __init__(self, seq_id, slot, num_groups):
         self.seq_id, self.slot = seq_id, slot
@@ -44,6 +50,15 @@ class SeqCache:
         self.num_pages = [0] * num_groups                # table entries filled (by page index)
         self.first_live = [0] * num_groups               # first page index not yet given back
         self.alive = True
+        self.family: Optional[Family] = None             # the beams it shares pages with
+
+
+class Family:
+    """What the beams of one prompt have in common: the first `shared` tokens lie on the same pages in every group that keeps all keys."""
+    __slots__ = ("shared",)
+
+    def __init__(self):
+        self.shared = 0
 
 
 class _Group:
@@ -237,6 +252,93 @@ class CacheManager:
         self.slots.release(seq.slot)
         del self.seqs[seq.seq_id]
 
+    # ---------------------------------------------------------------- beams
+    def fork(self, seq: SeqCache, seq_ids) -> Optional[List[SeqCache]]:
+        """A hold on the tokens of `seq` for every id, or None (and nothing taken) where pages or slots are short.  What the last page and the states
+        of the new ones hold is undefined until reorder gives them a parent."""
+        if not seq.alive or any(i in self.seqs for i in seq_ids) or len(set(seq_ids)) != len(list(seq_ids)):
+            raise RuntimeError(f"request {seq.seq_id!r} cannot be forked into {list(seq_ids)!r}")
+        full, part = divmod(seq.num_tokens, self.page_size)
+        if self.slots.num_free < len(seq_ids) or (part and any(g.pool.num_free < len(seq_ids) for g in self.kv_groups)):
+            return None
+        if seq.family is None:
+            seq.family = Family()
+        children = []
+        for i in seq_ids:
+            child = SeqCache(i, self.slots.claim(), len(self.kv_groups))
+            child.num_tokens, child.first_live, child.family = seq.num_tokens, list(seq.first_live), seq.family
+            for gi, g in enumerate(self.kv_groups):
+                child.num_pages[gi] = full + (part > 0)
+                for idx in self._live_pages(gi, child):
+                    if idx < full:
+                        page = int(g.tables[seq.slot, idx])
+                        g.pool.share(page)
+                    else:
+                        page = g.pool.take()
+                    self._set_entry(g, child.slot, idx, page)
+            self.seqs[i] = child
+            children.append(child)
+        self._measure_family([seq, *children])
+        return children
+
+    def _set_entry(self, g: _Group, slot: int, idx: int, page: int) -> None:
+        g.tables[slot, idx] = page
+        g.dirty[slot * self.max_pages_per_seq + idx] = None
+
+    def _measure_family(self, seqs) -> None:
+        """How many leading tokens lie on common pages."""
+        full = seqs[0].num_tokens // self.page_size
+        whole = next((g for g in self.kv_groups if g.need.window is None), None)
+        same = 0
+        if whole is not None and full:
+            rows = whole.tables[[s.slot for s in seqs], :full]
+            differ = (rows != rows[0]).any(axis=0)
+            same = int(differ.argmax()) if differ.any() else full
+        seqs[0].family.shared = same * self.page_size
+
+    def reorder(self, groups, ops) -> None:
+        """groups: [(beams of one prompt, a parent's place among them for each)].  Every beam then holds what its parent held.  The beams of a prompt
+        have cached the same number of tokens."""
+        moves = [([], [], [0]) for _ in range(len(self.kv_groups) + 1)]        # per kv group, and for the states: rows, parents (places in rows), group starts
+        for seqs, parents in groups:
+            if len(seqs) != len(parents) or any(not 0 <= p < len(seqs) for p in parents):
+                raise ValueError(f"{len(parents)} parents {list(parents)!r} for {len(seqs)} beams")
+            if any(s.num_tokens != seqs[0].num_tokens or s.family is not seqs[0].family or s.family is None or not s.alive for s in seqs):
+                raise RuntimeError("only beams of one prompt that have cached the same number of tokens take over one another's cache")
+            if all(p == i for i, p in enumerate(parents)):
+                continue
+            full, part = divmod(seqs[0].num_tokens, self.page_size)
+            for gi, g in enumerate(self.kv_groups):
+                old = g.tables[[s.slot for s in seqs], :full].copy()
+                shared = [idx for idx in self._live_pages(gi, seqs[0]) if idx < full]
+                moved = [(i, idx) for i, p in enumerate(parents) for idx in shared if old[i, idx] != old[p, idx]]
+                for i, idx in moved:                      # first all new holders, so that no page runs out of them in between
+                    g.pool.share(int(old[parents[i], idx]))
+                for i, idx in moved:
+                    g.pool.give(int(old[i, idx]))
+                    self._set_entry(g, seqs[i].slot, idx, int(old[parents[i], idx]))
+                if part:
+                    self._add_move(moves[gi], [int(g.tables[s.slot, full]) for s in seqs], parents)
+            self._add_move(moves[-1], [s.slot for s in seqs], parents)
+            self._measure_family(seqs)
+        tensors = [[(g.storage, 2)] + ([(g.value_storage, 1)] if g.value_storage is not None else []) for g in self.kv_groups]
+        tensors.append([(g.storage, 0) for g in self.state_groups])
+        for (rows, parents, start), held in zip(moves, tensors):
+            if not rows or not held:
+                continue
+            lists = torch.tensor(rows + parents + start, dtype=torch.int32)
+            lists = (lists.pin_memory() if self.device.type == "cuda" else lists).to(self.device, non_blocking=True)
+            n, most = len(rows), max(b - a for a, b in zip(start, start[1:]))
+            for dim in sorted({d for _, d in held}):
+                ops.reorder_rows([t for t, d in held if d == dim], lists[:n], lists[n:2 * n], lists[2 * n:], most, dim=dim)
+
+    @staticmethod
+    def _add_move(move, rows, parents) -> None:
+        first = len(move[0])
+        move[0].extend(rows)
+        move[1].extend(first + p for p in parents)
+        move[2].append(len(move[0]))
+
     # ---------------------------------------------------------------- what a step reads
     def slots_for(self, gi: int, seq: SeqCache, start: int, end: int) -> np.ndarray:
         """Flat cache positions page * page_size + offset of tokens start..end-1
@@ -269,7 +371,7 @@ class CacheManager:
 
     # ---------------------------------------------------------------- checks and numbers
     def check_invariants(self) -> None:
-        """No page lost, none held twice, free list and tables disjoint (used by the tests)."""
+        """No page lost, none held twice but full ones by beams, free list and tables disjoint (used by the tests)."""
         for gi, g in enumerate(self.kv_groups):
             held = []
             for seq in self.seqs.values():
@@ -288,13 +390,15 @@ class CacheManager:
                     mirror[k] = g.tables.reshape(-1)[k]
                 assert (mirror == g.tables.reshape(-1)).all(), f"group {gi}: device table differs beyond the noted changes"
             free = list(g.pool.free)
-            assert len(set(held)) == len(held), f"group {gi}: a page is held twice"
+            holders = Counter(held)
+            full = {int(p) for s in self.seqs.values() if s.family is not None for p in g.tables[s.slot, :s.num_tokens // self.page_size]}
+            assert all(n == 1 or p in full for p, n in holders.items()), f"group {gi}: a page that is not full is held twice"
             assert len(set(free)) == len(free), f"group {gi}: a page is in the free list twice"
             assert not set(held) & set(free), f"group {gi}: a held page is also free"
-            assert len(held) + len(free) == g.pool.num_pages, f"group {gi}: a page is lost"
+            assert len(holders) + len(free) == g.pool.num_pages, f"group {gi}: a page is lost"
             assert 0 not in free
             for p in range(1, g.pool.num_pages + 1):
-                assert g.pool.ref[p] == (1 if p in set(held) else 0)
+                assert g.pool.ref[p] == holders[p]
 
     def stats(self) -> dict:
         """Names after engine/core/kv_cache.py:283-301,427-437."""

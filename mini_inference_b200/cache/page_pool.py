@@ -37,7 +37,7 @@ class PagePool:
         return page
 
     def share(self, page: int) -> None:
-        """One more holder of a page in use (kept for prefix sharing; unused by the engine)."""
+        """One more holder of a page in use (beams share their common prefix's full pages)."""
         assert self.ref[page] > 0
         self.ref[page] += 1
 

@@ -50,7 +50,9 @@ class StepFacts:
     fed tokens, the position of the first, the keys it sees, its state slot.  This is what a
     part's step_arrays(facts) computes its own arrays from."""
 
-    def __init__(self, lens, pos0, slots, tile: int):
+    def __init__(self, lens, pos0, slots, tile: int, shared=None):
+        """shared: per entry (group, its first so many keys that the group's entries have in common), or None where a step has no beams."""
+        self.shared = shared
         self.lens = np.asarray(lens, dtype=np.int32)
         self.pos0 = np.asarray(pos0, dtype=np.int32)
         self.slots = np.asarray(slots, dtype=np.int32)
@@ -90,8 +92,23 @@ class GroupView:
         return getattr(self.__dict__["batch"], name)
 
 
+def shared_of(seqs, lens):
+    """Per entry the group of beams that it feeds one token beside, and their common first keys (StepFacts.shared); None without beams."""
+    if all(s.family is None for s in seqs):
+        return None
+    out, at, last = [], -1, None
+    for s, n in zip(seqs, lens):
+        family = s.family if n == 1 else None
+        if family is None or family is not last:
+            at += 1
+        last = family
+        out.append((at, 0 if family is None else family.shared))
+    return out
+
+
 class StepBatch:
     """Device views of one step's fields, plus the host-side facts."""
+    shared_start = None             # steps with beams have it among the paged attention's arrays
 
     def __init__(self, layout: BatchLayout, dev: torch.Tensor, cache, facts: StepFacts, shapes: dict,
                  num_logit_rows: int, max_kv_len: int, sampling: bool):
@@ -101,6 +118,8 @@ class StepBatch:
         self.max_kv_len, self.max_q_len = max_kv_len, int(facts.lens.max())
         prompts = facts.lens > 1                                    # entries that feed more than one token; the most keys one of them sees
         self.max_prompt_kv_len = int(facts.kv_len[prompts].max()) if prompts.any() else 0
+        groups = [0] if facts.shared is None else np.unique([g for g, _ in facts.shared], return_counts=True)[1]
+        self.max_shared_rows = int(max(groups))
         self.host = {"seg_q_start": facts.q_start, "seg_pos0": facts.pos0, "seg_kv_len": facts.kv_len,
                      "seg_slot": facts.slots.tolist(), "lens": facts.lens}
         for name in ("token_ids", "positions", "token_seg", "seg_q_start", "seg_pos0", "seg_kv_len", "seg_slot", "logit_rows"):
@@ -252,7 +271,7 @@ class BatchBuilder:
     def build(self, entries: List[StepEntry]) -> StepBatch:
         """The batch of an eager step: fields sized to the step, a fresh device buffer, one copy."""
         lens = [len(e.tokens) for e in entries]
-        facts = StepFacts(lens, [e.seq.num_tokens for e in entries], [e.seq.slot for e in entries], self.tile)
+        facts = StepFacts(lens, [e.seq.num_tokens for e in entries], [e.seq.slot for e in entries], self.tile, shared_of([e.seq for e in entries], lens))
         ids = np.fromiter((t for e in entries for t in e.tokens), dtype=np.int64, count=facts.num_tokens)
         self._check_tokens(ids)
         rows = np.asarray([int(facts.q_start[i]) + w for i, e in enumerate(entries) for w in e.want], dtype=np.int32)

@@ -17,6 +17,7 @@ from ..cache.manager import CacheManager
 from ..config.engine_args import EngineArgs
 from ..sampling.sampler import Sampler
 from .batch import StepEntry
+from .beam import Beam, BeamParams, BeamSearch
 from .factory import DTYPES, load_model
 from .request import RUNNING, Request, SamplingParams
 from .runner import ModelRunner
@@ -119,12 +120,16 @@ class LLM:
         return max(int(max(budget, 0) // max(bytes_per_token, 1)), 1024)
 
     # ---------------------------------------------------------------- requests
-    def add_request(self, prompt_ids: Sequence[int], params: Optional[SamplingParams] = None) -> Request:
+    def _checked_prompt(self, prompt_ids: Sequence[int]) -> List[int]:
         ids = [int(t) for t in prompt_ids]
         if not ids:
             raise ValueError("the prompt is empty")                       # engine/custom_engine.py:189-190
         if min(ids) < 0 or max(ids) >= self.model.spec.vocab_size:
             raise ValueError(f"token id outside [0, {self.model.spec.vocab_size})")
+        return ids
+
+    def add_request(self, prompt_ids: Sequence[int], params: Optional[SamplingParams] = None) -> Request:
+        ids = self._checked_prompt(prompt_ids)
         limit = min(self.max_model_len, self.cache.capacity_tokens)
         if len(ids) >= limit:
             raise ValueError(f"prompt is {len(ids)} tokens; the limit is {limit - 1}")   # :191-193
@@ -290,6 +295,25 @@ class LLM:
         if hasattr(self.ops, "check_errors"):
             self.ops.check_errors()                    # a bounded wait inside a kernel ran out: the tokens cannot be trusted
         return [list(r.output_ids) for r in reqs]
+
+    def beam_search(self, prompts: Sequence[Sequence[int]], params: Optional[BeamParams] = None) -> List[List[Beam]]:
+        """Token ids in; per prompt its num_beams best continuations, best first.  Runs by itself: requests that were added by add_request come first.  A prompt
+        whose beams do not fit beside one another in the cache raises CacheFull."""
+        if self.has_work():
+            raise RuntimeError("beam_search runs by itself: step() until has_work() is False")
+        params = params or BeamParams(max_new_tokens=self.args.max_new_tokens)
+        ids = [self._checked_prompt(p) for p in prompts]
+        limit = min(self.max_model_len, self.cache.capacity_tokens)
+        for p in ids:
+            if len(p) + params.max_new_tokens > limit:
+                raise ValueError(f"prompt is {len(p)} tokens and {params.max_new_tokens} more are wanted; the limit is {limit}")
+        if params.num_beams > self.args.max_num_seqs:
+            raise ValueError(f"{params.num_beams} beams; the engine holds {self.args.max_num_seqs} sequences")
+        with torch.inference_mode():
+            out = BeamSearch(self).run(ids, params)
+        if hasattr(self.ops, "check_errors"):
+            self.ops.check_errors()
+        return out
 
     def score(self, token_ids: Sequence[int]) -> torch.Tensor:
         """float32 logits for every position, through the paged cache (engine/custom_engine.py:279-296)."""

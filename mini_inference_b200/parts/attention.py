@@ -18,14 +18,19 @@ from .base import KVCacheNeed, Part, WeightSpec, register_mixer
 def paged_attention_step_arrays(facts):
     """The paged attention kernels' work lists (shared by every mixer whose step_arrays_key is "paged_attention"): the
     entries that feed one token (decode kernels), and for the longer entries one (entry, first row) pair per tile of
-    query rows (prompt kernels; the tensor-core kernel takes tiles twice as tall)."""
+    query rows (prompt kernels; the tensor-core kernel takes tiles twice as tall).  Steps with beams: which decoded tokens share their first keys."""
     lens, tile = facts.lens, facts.tile
     decode = [i for i, n in enumerate(lens) if n == 1]
     tiles = [(i, r) for i, n in enumerate(lens) if n > 1 for r in range(0, n, tile)]
     tiles2 = [(i, r) for i, n in enumerate(lens) if n > 1 for r in range(0, n, 2 * tile)]
     as_i32 = lambda v, shape: np.asarray(v, dtype=np.int32).reshape(shape)      # noqa: E731
-    return {"decode_segs": as_i32(decode, (-1,)), "prefill_tiles": as_i32(tiles, (-1, 2)),
-            "prefill_tiles2": as_i32(tiles2, (-1, 2))}
+    arrays = {"decode_segs": as_i32(decode, (-1,)), "prefill_tiles": as_i32(tiles, (-1, 2)),
+              "prefill_tiles2": as_i32(tiles2, (-1, 2))}
+    if facts.shared is not None and decode:              # beams: groups of neighbours in decode_segs, the keys that a group's entries have in common
+        groups = [facts.shared[i] for i in decode]
+        first = [i for i, g in enumerate(groups) if i == 0 or g[0] != groups[i - 1][0]]
+        arrays["shared_start"], arrays["shared_len"] = as_i32(first + [len(decode)], (-1,)), as_i32([groups[i][1] for i in first], (-1,))
+    return arrays
 
 
 @register_mixer("gqa_attention")
