@@ -22,18 +22,23 @@ constexpr int MAX_ENTITIES = 4096;                   // groups + rows of a call
 
 struct Args {
     const int *decode_segs, *seg_q_start, *seg_kv_len, *block_table, *table_rows, *shared_start, *shared_len;
-    int R, G, most, table_stride, H, KV, ps;           // most: rows of the largest group; rows beyond it have no prefix part
+    int R, G, entries, most, table_stride, H, KV, ps;  // most: rows of the largest group; rows beyond it have no prefix part
     int row_tiles, tile_rows;                        // tiles of rows of the largest group; rows of a tile (x H / KV heads = its matrix rows)
-    int slot_rows;                                   // matrix rows of a prefix piece's place
-    float *o_prefix, *o_tail;                        // [places][D / 4][slot_rows or H / KV][4], not divided by the sums: neighbouring rows' 16 bytes side by side
-    float2 *ml_prefix, *ml_tail;                     // [places][slot_rows or H / KV]: maximum (base 2) and sum
+    int copies;                                      // 1: a piece's keys may be shared out over up to 4 copies of its rows (see copies_of)
+    int slot_rows, tail_rows;                        // rows of a prefix piece's place and of a tail piece's, copies among them
+    float *o_prefix, *o_tail;                        // [places][D / 4][rows of a place][4], not divided by the sums: neighbouring rows' 16 bytes side by side
+    float2 *ml_prefix, *ml_tail;                     // [places][rows of a place]: maximum (base 2) and sum
     int* plan;                                       // what block 0 leaves for the merge: tiles of a block, and a Record per row
 };
 
 struct __align__(16) Record {                        // where a row's pieces are: its token; the prefix item of key head 0 (first tile, tiles to the next key head's,
     int token, prefix_at, prefix_step, prefix_tiles; // tiles, place, first matrix row) and the tail's (first tile, tiles)
-    int prefix_place, prefix_row, tail_at, tail_tiles;
+    int prefix_place, prefix_row, tail_at, tail_tiles;      // prefix_row: the tile's rows in the upper half
 };
+
+// How often a piece of so many rows has each of them: the copies' keys are different columns of a tile, so each is a piece of its own to the merge.
+// Copy s of row i is row s rows + i of the piece's place.
+__host__ __device__ __forceinline__ int copies_of(int copies, int rows) { return !copies || rows > 64 ? 1 : rows > 32 ? 2 : 4; }
 
 // in shared memory: sums of tiles [G + R + 1]; a row's first tail key, group (-1: none), keys, token and row of the block table [R] each; a group's first row, rows,
 // shared keys and the row whose pages hold them [G] each
@@ -62,10 +67,13 @@ __device__ __forceinline__ void make_plan(const Args& a, const Plan& p) {
         p.sums[g + 1] = a.KV * ((n + a.tile_rows - 1) / a.tile_rows) * with_pad((keys + KT - 1) / KT);
     }
     for (int r = threadIdx.x; r < a.R; r += blockDim.x) {
-        const int seg = a.decode_segs[r];
-        p.keys[r] = min(a.seg_kv_len[seg], a.table_stride * a.ps);
-        p.token[r] = a.seg_q_start[seg];
-        p.table[r] = a.table_rows ? a.table_rows[seg] : seg;
+        // entry r is most often entry decode_segs[r]: its numbers are asked for beside it, not behind it
+        const int guess = min(r, a.entries - 1), seg = a.decode_segs[r];
+        int keys = a.seg_kv_len[guess], token = a.seg_q_start[guess], row = a.table_rows ? a.table_rows[guess] : guess;
+        if (seg != guess) { keys = a.seg_kv_len[seg]; token = a.seg_q_start[seg]; row = a.table_rows ? a.table_rows[seg] : seg; }
+        p.keys[r] = min(keys, a.table_stride * a.ps);
+        p.token[r] = token;
+        p.table[r] = row;
     }
     __syncthreads();
     for (int r = threadIdx.x; r < a.R; r += blockDim.x) {
@@ -103,7 +111,7 @@ __device__ __forceinline__ void make_plan(const Args& a, const Plan& p) {
                 rec.prefix_at = p.sums[g] + mt * rec.prefix_tiles;
                 rec.prefix_step = tm * rec.prefix_tiles;
                 rec.prefix_place = g * a.KV * a.row_tiles + mt;
-                rec.prefix_row = (r - start) % a.tile_rows * (a.H / a.KV);
+                rec.prefix_row = (r - start) % a.tile_rows * (a.H / a.KV) | min(a.tile_rows, p.rows[g] - mt * a.tile_rows) * (a.H / a.KV) << 16;
             }
             records[r] = rec;
         }
@@ -168,74 +176,90 @@ struct Walk {
 // out[token of row r, heads of key head] from the row's pieces: a block per (row, key head), as many heads at a time as fill 128 threads with four columns each
 // (neighbouring heads in neighbouring threads).  A warp per head makes the weights of all pieces, then MERGE_PARTS groups of 128 threads take every
 // MERGE_PARTS-th piece, their rows read without waiting for one another, and are added up in the groups' order.
-constexpr int MERGE_PARTS = 4, MERGE_PIECES = 1280;  // pieces of a row at most: one a block for its prefix, one for its tail
+constexpr int MERGE_PARTS = 4, MERGE_PIECES = 512;   // pieces whose weights are made at a time
 template <typename T, int D>
 __global__ void __launch_bounds__(128 * MERGE_PARTS) merge_kernel(const __grid_constant__ Args a, T* __restrict__ out) {
     constexpr int HEADS = 512 / D;
-    __shared__ float weight[MERGE_PIECES * HEADS], inverse[HEADS];
+    __shared__ float weight[MERGE_PIECES * HEADS], keep[HEADS], total[HEADS];
     __shared__ float4 parts[MERGE_PARTS - 1][128];
     pdl_trigger();
     pdl_wait(out);
     const int r = blockIdx.x, kvh = blockIdx.y, Hg = a.H / a.KV, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int per = a.plan[0];
     const Record rec = reinterpret_cast<const Record*>(a.plan + 4)[r];
-    int n_p = 0, n_t = 0;                            // pieces of the prefix, then of the tail; their places follow on one another
+    // pieces of the prefix, then of the tail, every copy of the row one of them; a part's places follow on one another
+    const int rows_p = rec.prefix_row >> 16, copies_p = copies_of(a.copies, rows_p), copies_t = copies_of(a.copies, Hg);
+    const int shift_p = copies_p >> 1, shift_t = copies_t >> 1;        // log2 of 1, 2, 4
+    int n_p = 0, n_t = 0;
     size_t at_p = 0, at_t = 0;
     if (rec.prefix_tiles > 0) {
         const int t0 = rec.prefix_at + kvh * rec.prefix_step;
-        n_p = (t0 + rec.prefix_tiles - 1) / per - (t0 + PAD) / per + 1;
+        n_p = ((t0 + rec.prefix_tiles - 1) / per - (t0 + PAD) / per + 1) << shift_p;
         at_p = (size_t)rec.prefix_place + (size_t)kvh * a.row_tiles + (t0 + PAD) / per;
     }
     if (rec.tail_tiles > 0) {
         const int t0 = rec.tail_at + kvh * rec.tail_tiles;
-        n_t = (t0 + rec.tail_tiles - 1) / per - (t0 + PAD) / per + 1;
+        n_t = ((t0 + rec.tail_tiles - 1) / per - (t0 + PAD) / per + 1) << shift_t;
         at_t = (size_t)r * a.KV + kvh + (t0 + PAD) / per;
     }
-    n_p = min(n_p, MERGE_PIECES / 2);
-    const int n = n_p + min(n_t, MERGE_PIECES / 2);
+    const int n = n_p + n_t;
     for (int h0 = 0; h0 < Hg; h0 += HEADS) {
-        const int heads = min(HEADS, Hg - h0);
-        if (warp < heads) {
-            const float2 *p = a.ml_prefix + at_p * a.slot_rows + rec.prefix_row + h0 + warp, *q = a.ml_tail + at_t * Hg + h0 + warp;
-            const auto piece = [&](int i) { return i < n_p ? p[(size_t)i * a.slot_rows] : q[(size_t)(i - n_p) * Hg]; };
-            const float2 first = lane < n ? piece(lane) : make_float2(-INFINITY, 0.f);
-            float m = first.x, l = 0.f;
-            for (int i = lane + 32; i < n; i += 32) m = fmaxf(m, piece(i).x);
-            m = warp_max(m);
-            const float off = m == -INFINITY ? 0.f : m;               // -inf: none of a piece's keys is visible to this row
-            for (int i = lane; i < n; i += 32) {
-                const float2 ml = i < 32 ? first : piece(i);
-                const float w = exp2f(ml.x - off);
-                weight[i * HEADS + warp] = w;
-                if (w != 0.f) l = fmaf(ml.y, w, l);
-            }
-            l = warp_sum(l);
-            if (lane == 0) inverse[warp] = l > 0.f ? 1.f / l : l == 0.f ? 0.f : l;      // no key at all: 0; NaN stays
-        }
-        __syncthreads();
-        const int id = threadIdx.x & 127, part = threadIdx.x >> 7, h = id % heads, c = id / heads;
+        const int heads = min(HEADS, Hg - h0), id = threadIdx.x & 127, part = threadIdx.x >> 7, h = id % heads, c = id / heads;
         const bool mine = c < D / 4;
+        const int row_p = (rec.prefix_row & 0xffff) + h0, row_t = h0;
+        float m = -INFINITY, l = 0.f;                // of this warp's head
         float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-        const auto add = [&](const float4& v, float w) {              // a weight of 0: what a piece without visible keys holds counts for nothing
-            o.x = w == 0.f ? o.x : fmaf(v.x, w, o.x); o.y = w == 0.f ? o.y : fmaf(v.y, w, o.y);
-            o.z = w == 0.f ? o.z : fmaf(v.z, w, o.z); o.w = w == 0.f ? o.w : fmaf(v.w, w, o.w);
-        };
-        if (mine) {
-            const float4* p = reinterpret_cast<const float4*>(a.o_prefix) + (at_p * (D / 4) + c) * a.slot_rows + rec.prefix_row + h0 + h;
-            const float4* q = reinterpret_cast<const float4*>(a.o_tail) + (at_t * (D / 4) + c) * Hg + h0 + h;
-            const size_t step_p = (size_t)(D / 4) * a.slot_rows, step_q = (size_t)(D / 4) * Hg;
-            int i = part;
+        for (int i0 = 0; i0 < max(n, 1); i0 += MERGE_PIECES) {
+            const int now = min(MERGE_PIECES, n - i0);
+            if (warp < heads) {
+                const auto piece = [&](int i) {
+                    i += i0;
+                    if (i < n_p) return a.ml_prefix[(at_p + (i >> shift_p)) * a.slot_rows + (i & (copies_p - 1)) * rows_p + row_p + warp];
+                    i -= n_p;
+                    return a.ml_tail[(at_t + (i >> shift_t)) * a.tail_rows + (i & (copies_t - 1)) * Hg + row_t + warp];
+                };
+                const float2 first = lane < now ? piece(lane) : make_float2(-INFINITY, 0.f);
+                float top = fmaxf(m, first.x);
+                for (int i = lane + 32; i < now; i += 32) top = fmaxf(top, piece(i).x);
+                top = warp_max(top);
+                const float off = top == -INFINITY ? 0.f : top, old = exp2f(m - off);      // -inf: none of a piece's keys is visible to this row
+                float sum = 0.f;
+                for (int i = lane; i < now; i += 32) {
+                    const float2 ml = i < 32 ? first : piece(i);
+                    const float w = exp2f(ml.x - off);
+                    weight[i * HEADS + warp] = w;
+                    if (w != 0.f) sum = fmaf(ml.y, w, sum);
+                }
+                m = top;
+                l = l * old + warp_sum(sum);
+                if (lane == 0) { keep[warp] = old; total[warp] = l; }
+            }
+            __syncthreads();
+            if (mine) {
+                const float old = keep[h];
+                o.x *= old; o.y *= old; o.z *= old; o.w *= old;
+                const auto add = [&](const float4& v, float w) {      // a weight of 0: what a piece without visible keys holds counts for nothing
+                    o.x = w == 0.f ? o.x : fmaf(v.x, w, o.x); o.y = w == 0.f ? o.y : fmaf(v.y, w, o.y);
+                    o.z = w == 0.f ? o.z : fmaf(v.z, w, o.z); o.w = w == 0.f ? o.w : fmaf(v.w, w, o.w);
+                };
+                const float4* p = reinterpret_cast<const float4*>(a.o_prefix) + (at_p * (D / 4) + c) * a.slot_rows + row_p + h;
+                const float4* q = reinterpret_cast<const float4*>(a.o_tail) + (at_t * (D / 4) + c) * a.tail_rows + row_t + h;
+                const size_t step_p = (size_t)(D / 4) * a.slot_rows, step_q = (size_t)(D / 4) * a.tail_rows;
+                int i = i0 + part;
+                const int end = i0 + now, end_p = min(n_p, end);
 #pragma unroll 4
-            for (; i < n_p; i += MERGE_PARTS) add(p[i * step_p], weight[i * HEADS + h]);
+                for (; i < end_p; i += MERGE_PARTS) add(p[(i >> shift_p) * step_p + (i & (copies_p - 1)) * rows_p], weight[(i - i0) * HEADS + h]);
 #pragma unroll 2
-            for (; i < n; i += MERGE_PARTS) add(q[(i - n_p) * step_q], weight[i * HEADS + h]);
+                for (; i < end; i += MERGE_PARTS) add(q[((i - n_p) >> shift_t) * step_q + ((i - n_p) & (copies_t - 1)) * Hg], weight[(i - i0) * HEADS + h]);
+            }
+            __syncthreads();
         }
         if (part) parts[part - 1][id] = o;
         __syncthreads();
         if (part == 0 && mine) {
 #pragma unroll
             for (int k = 0; k < MERGE_PARTS - 1; ++k) { const float4 v = parts[k][id]; o.x += v.x; o.y += v.y; o.z += v.z; o.w += v.w; }
-            const float inv = inverse[h];
+            const float sum = total[h], inv = sum > 0.f ? 1.f / sum : sum == 0.f ? 0.f : sum;      // no key at all: 0; NaN stays
             T* to = out + ((size_t)rec.token * a.H + (size_t)kvh * Hg + h0 + h) * D + 4 * c;
             store2(to, o.x * inv, o.y * inv);
             store2(to + 2, o.z * inv, o.w * inv);
@@ -244,17 +268,27 @@ __global__ void __launch_bounds__(128 * MERGE_PARTS) merge_kernel(const __grid_c
     }
 }
 
+// Lets a kernel have `bytes` of shared memory, once a device (asking again costs a call about 2 us)
+template <typename Kernel> inline cudaError_t allow_shared(Kernel kernel, int bytes, unsigned long long& devices_done) {
+    int dev = 0;
+    cudaError_t e = cudaGetDevice(&dev);
+    if (e != cudaSuccess || (dev < 64 && devices_done >> dev & 1)) return e;
+    e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+    if (e == cudaSuccess && dev < 64) devices_done |= 1ull << dev;
+    return e;
+}
+
 // Scratch of a call: floats of o_prefix, o_tail, then float2 of both, then the plan
 struct Scratch { long long o_prefix, o_tail, ml_prefix, ml_tail, plan, bytes; };
-inline Scratch scratch(int R, int G, int H, int KV, int D, int row_tiles, int slot_rows, int blocks) {
-    const long long places_p = (long long)G * KV * row_tiles + blocks, places_t = (long long)R * KV + blocks, Hg = H / KV;
+inline Scratch scratch(int R, int G, int KV, int D, int row_tiles, int slot_rows, int tail_rows, int blocks) {
+    const long long places_p = (long long)G * KV * row_tiles + blocks, places_t = (long long)R * KV + blocks;
     const auto up = [](long long v) { return (v + 255) / 256 * 256; };
     Scratch s;
     s.o_prefix = 0;
     s.o_tail = s.o_prefix + up(places_p * slot_rows * D * 4);
-    s.ml_prefix = s.o_tail + up(places_t * Hg * D * 4);
+    s.ml_prefix = s.o_tail + up(places_t * tail_rows * D * 4);
     s.ml_tail = s.ml_prefix + up(places_p * slot_rows * 8);
-    s.plan = s.ml_tail + up(places_t * Hg * 8);
+    s.plan = s.ml_tail + up(places_t * tail_rows * 8);
     s.bytes = s.plan + up(16 + (long long)R * sizeof(Record));
     return s;
 }

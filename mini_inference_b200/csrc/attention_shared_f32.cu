@@ -172,24 +172,25 @@ int slot_rows_of(int H, int KV, int most) { const int t = tile_rows_of(H, KV); r
 // Bytes of the work space of a call; -2: sizes that this kernel does not take.  most: rows of the largest group.
 MI_EXPORT long long mi_attn_shared_f32_bytes(int R, int G, int most, int H, int KV, int D, int ps) {
     if (!fits(R, G, H, KV, D, ps)) return -2;
-    return scratch(R, G, H, KV, D, row_tiles_of(H, KV, most), slot_rows_of(H, KV, most), 2 * device_sms()).bytes;
+    return scratch(R, G, KV, D, row_tiles_of(H, KV, most), slot_rows_of(H, KV, most), H / KV, 2 * device_sms()).bytes;
 }
 
 // As mi_attn_shared_tc, in float32.
 MI_EXPORT int mi_attn_shared_f32(const float* q, int q_stride, const float* k_cache, const float* v_cache, float* out, const int* decode_segs, int R,
-                                 const int* seg_q_start, const int* seg_kv_len, const int* block_table, const int* table_rows, int table_stride,
+                                 const int* seg_q_start, const int* seg_kv_len, int entries, const int* block_table, const int* table_rows, int table_stride,
                                  const int* shared_start, const int* shared_len, int G, int most, int H, int KV, int D, int ps, float scale, void* work,
                                  cudaStream_t stream) {
     if (R == 0) return 0;
-    if (!fits(R, G, H, KV, D, ps) || q_stride % 4 || (((uintptr_t)q | (uintptr_t)k_cache | (uintptr_t)v_cache | (uintptr_t)work) % 16)) return -2;
+    if (!fits(R, G, H, KV, D, ps) || entries < 1 || q_stride % 4 || (((uintptr_t)q | (uintptr_t)k_cache | (uintptr_t)v_cache | (uintptr_t)work) % 16)) return -2;
     const int blocks = 2 * device_sms();
-    Args a{decode_segs, seg_q_start, seg_kv_len, block_table, table_rows, shared_start, shared_len, R, G, most > 1 ? most : 1, table_stride, H, KV, ps,
-           row_tiles_of(H, KV, most), tile_rows_of(H, KV), slot_rows_of(H, KV, most)};
-    place_scratch(a, scratch(R, G, H, KV, D, a.row_tiles, a.slot_rows, blocks), work);
+    Args a{decode_segs, seg_q_start, seg_kv_len, block_table, table_rows, shared_start, shared_len, R, G, entries, most > 1 ? most : 1, table_stride, H, KV, ps,
+           row_tiles_of(H, KV, most), tile_rows_of(H, KV), 0, slot_rows_of(H, KV, most), H / KV};
+    place_scratch(a, scratch(R, G, KV, D, a.row_tiles, a.slot_rows, a.tail_rows, blocks), work);
     const float scale_log2 = scale * 1.4426950408889634f;
 #define LAUNCH(DD) do { \
         const size_t smem = (size_t)Tiles<DD>::END * 4, plan = (size_t)plan_ints(G, R) * 4; \
-        cudaError_t e = cudaFuncSetAttribute(attn_shared_f32_kernel<DD>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)(smem + (6 * MAX_ENTITIES + 1) * 4)); \
+        static unsigned long long done = 0; \
+        cudaError_t e = allow_shared(attn_shared_f32_kernel<DD>, (int)(smem + (6 * MAX_ENTITIES + 1) * 4), done); \
         if (e == cudaSuccess) e = launch_pdl(attn_shared_f32_kernel<DD>, dim3(blocks), dim3(THREADS), smem + plan, stream, a, q, (long long)q_stride, k_cache, v_cache, \
                                              scale_log2); \
         if (e == cudaSuccess) e = launch_pdl(merge_kernel<float, DD>, dim3(R, KV), dim3(128 * MERGE_PARTS), 0, stream, a, out); \

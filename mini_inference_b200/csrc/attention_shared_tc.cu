@@ -5,13 +5,18 @@
 // of one key head, 128 / (H / KV) rows; a tail has the H / KV heads of its row.  Lanes beyond them hold whatever was there and write nothing.
 //
 // One block is seven warps, two blocks an SM; a block walks its tiles of 64 keys through all its pieces without a stop:
-//   warp 0, 6  TMA: key and value tiles, box by box of the page table's rows, into rings of two tiles (128-byte swizzle).  They run ahead over
-//              the end of a piece.  A tile with values in front of a piece's first or behind its last key arrives on a barrier of its own, is cleared
-//              there (what lies in a page's unused part may be anything, and 0 * inf is no 0) and handed on.
-//   warp 1     one thread issues S = Q K^T (scores in one of two 64-column buffers of tensor memory) a tile ahead, and O += P V
+//   warp 0     queries (TMA, a box of heads per row) and key tiles (TMA, box by box of the page table's rows) into a ring of two, 128-byte swizzle; runs
+//              ahead over the end of a piece, and asks the page table for a tile while the one before waits for its place
+//   warp 6     value tiles, the same way
+//   warp 1     one thread issues S = Q K^T (scores in one of two 64-column buffers of tensor memory) up to a tile ahead, over the end of a piece too, and
+//              O += P V, whichever has its operands first
 //   warps 2-5  a matrix row a thread: mask, running maximum and sum (float32, base 2; the exponent's offset is kept until the maximum has grown by 2^8),
-//              weights as bfloat16 back to tensor memory; values that no row sees are cleared in shared memory.  With the last tile's weights handed over they bring the next piece's queries, then write
-//              this one's O, maximum and sum.  A warp whose 32 rows are all beyond the piece only keeps step.
+//              weights as bfloat16 back to tensor memory; values that no row sees are cleared in shared memory (what lies in a page's unused part may be
+//              anything, and 0 * inf is no 0).  At the end of a piece they write its O, maximum and sum.
+// A warp reaches 32 rows of tensor memory, so with few rows one warp would make all weights while three wait (64 exponentials a thread are 512 clocks).
+// Up to 32 rows therefore stand in the tile four times, up to 64 twice, and each copy's warps take their own part of the 64 columns, the others' weights
+// being 0: a copy is a piece of its own with its own maximum and sum, so the warps need not agree on anything, and the merge adds copies like pieces.
+// Pieces of up to 16 rows use the two halves of their 32 rows in turn, so the next one's queries come while this one's products run.
 // Weights are rounded to bfloat16 for P V (2^-9 of each, of random sign over the keys; the sums take them unrounded), as the engine's other decode and prompt attention does.
 // Two launches: this one, and the merge.  Every mbarrier wait is bounded.
 #include "attention_shared.cuh"
@@ -46,10 +51,87 @@ __device__ __forceinline__ uint32_t pack_bf16(float a, float b) {
     return *reinterpret_cast<uint32_t*>(&v);
 }
 
+__device__ __forceinline__ void tma_load_3d(uint32_t dst, const CUtensorMap* map, int x, int y, int z, uint32_t bar) {
+    asm volatile("cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];\n"
+                 :: "r"(dst), "l"((uint64_t)map), "r"(x), "r"(y), "r"(z), "r"(bar) : "memory");
+}
+__device__ __forceinline__ void tmem_ld16(uint32_t taddr, uint32_t (&r)[16]) {
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];\n"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
+                   "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+                 : "r"(taddr) : "memory");
+}
+__device__ __forceinline__ void tmem_st8(uint32_t taddr, const uint32_t (&r)[8]) {
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};\n"
+                 :: "r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]) : "memory");
+}
+template <int W> __device__ __forceinline__ void tmem_ld(uint32_t taddr, uint32_t (&r)[W]) { if constexpr (W == 32) tmem_ld32(taddr, r); else tmem_ld16(taddr, r); }
+template <int W> __device__ __forceinline__ void tmem_st(uint32_t taddr, const uint32_t (&r)[W]) { if constexpr (W == 16) tmem_st16(taddr, r); else tmem_st8(taddr, r); }
+
+// A matrix row's scores of one tile, its columns col .. col + W parts - 1, to weights; the other columns' weights become 0
+struct Row { float m, l; };                          // the exponent's offset (base 2) and the sum of weights
+template <int W>
+__device__ __forceinline__ bool weights(uint32_t s_addr, int col, int parts, bool whole, uint32_t from, uint32_t span, float scale_log2, bool first, Row& row, float& alpha) {
+    uint32_t r[W];
+    const auto scores = [&](int part) {
+        tmem_ld<W>(s_addr + col + W * part, r);
+        tmem_wait_ld();
+        if (!whole) {
+#pragma unroll
+            for (int c = 0; c < W; ++c) r[c] = from + (part * W + c) < span ? r[c] : 0xff800000u;       // -inf
+        }
+    };
+    float mx4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll 1
+    for (int part = parts - 1; part >= 0; --part) {
+        scores(part);
+#pragma unroll
+        for (int c = 0; c < W; c += 8)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) mx4[e] = max3(mx4[e], __uint_as_float(r[c + 2 * e]), __uint_as_float(r[c + 2 * e + 1]));
+    }
+    const float mx = fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3])) * scale_log2;      // scale > 0
+    bool rescale = false;
+    alpha = 1.f;
+    if (mx > row.m + 8.f) {
+        alpha = row.m == -INFINITY ? 0.f : fast_exp2(row.m - mx);
+        rescale = !first && row.m != -INFINITY;
+        row.m = mx;
+        row.l *= alpha;
+    }
+    const float off = row.m == -INFINITY ? 0.f : row.m;
+    const float2 scale2 = make_float2(scale_log2, scale_log2), noff2 = make_float2(-off, -off);
+    float2 sums[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
+#pragma unroll 1
+    for (int part = 0; part < parts; ++part) {       // r holds the first part
+        if (part) scores(part);
+        uint32_t pk[W / 2];
+#pragma unroll
+        for (int c = 0; c < W / 2; ++c) {
+            const float2 arg = __ffma2_rn(make_float2(__uint_as_float(r[2 * c]), __uint_as_float(r[2 * c + 1])), scale2, noff2);
+            const float2 p = make_float2(fast_exp2(arg.x), fast_exp2(arg.y));
+            sums[c & 1] = __fadd2_rn(sums[c & 1], p);
+            pk[c] = pack_bf16(p.x, p.y);
+        }
+        tmem_st<W / 2>(s_addr + (col + W * part) / 2, pk);             // weights take the place of the first scores
+    }
+    const float2 s01 = __fadd2_rn(sums[0], sums[1]);
+    row.l += s01.x + s01.y;
+    uint32_t none[W / 2];
+#pragma unroll
+    for (int c = 0; c < W / 2; ++c) none[c] = 0u;
+    if (W * parts < KT) {
+#pragma unroll 1
+        for (int c = 0; c < KT; c += W)
+            if (c != col) tmem_st<W / 2>(s_addr + c / 2, none);
+    }
+    return rescale;
+}
+
 template <int D>
 __global__ void __launch_bounds__(THREADS, 2)
-attn_shared_tc_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap, const __grid_constant__ Args a,
-                      const __nv_bfloat16* __restrict__ q, long long q_stride, float scale_log2, int* __restrict__ error_word) {
+attn_shared_tc_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap,
+                      const __grid_constant__ Args a, float scale_log2, int* __restrict__ error_word) {
     constexpr int HALVES = D / 64, Q_BYTES = BQ * D * 2, KV_BYTES = KT * D * 2;
     constexpr int TMEM_COLS = 256;                       // S0: 64, S1: 64 (P takes the first 32 columns of its S), O: D
     constexpr uint32_t S_COL = 0, O_COL = 128;
@@ -57,29 +139,27 @@ attn_shared_tc_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_con
     unsigned char* base = (unsigned char*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
     // [Q][K0][K1][V0][V1][barriers][plan]
     uint64_t* bars = reinterpret_cast<uint64_t*>(base + Q_BYTES + 4 * KV_BYTES);
-    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 15);
-    const Plan plan(reinterpret_cast<int*>(bars + 16), a.G, a.R);
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 17);
+    const Plan plan(reinterpret_cast<int*>(bars + 18), a.G, a.R);
     const uint32_t sQ = smem_u32(base), sK = sQ + Q_BYTES, sV = sK + 2 * KV_BYTES;
-    const uint32_t q_full = smem_u32(bars), k_full = smem_u32(bars + 1), k_empty = smem_u32(bars + 3), s_full = smem_u32(bars + 5),
-                   p_ready = smem_u32(bars + 7), pv_done = smem_u32(bars + 8), v_full = smem_u32(bars + 9), v_empty = smem_u32(bars + 11),
-                   o_free = smem_u32(bars + 13);
+    // pairs: of tiles or pieces in turn
+    const uint32_t q_full = smem_u32(bars), q_done = smem_u32(bars + 2), k_full = smem_u32(bars + 4), k_empty = smem_u32(bars + 6), s_full = smem_u32(bars + 8),
+                   v_full = smem_u32(bars + 10), v_empty = smem_u32(bars + 12), p_ready = smem_u32(bars + 14), pv_done = smem_u32(bars + 15), o_free = smem_u32(bars + 16);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int Hg = a.H / a.KV;
 
     if (threadIdx.x == 0) {
-        mbar_init(q_full, 128);
-        mbar_init(k_full, 1); mbar_init(k_full + 8, 1); mbar_init(k_empty, 1); mbar_init(k_empty + 8, 1);
-        mbar_init(v_full, 1); mbar_init(v_full + 8, 1); mbar_init(v_empty, 1); mbar_init(v_empty + 8, 1);
-        mbar_init(s_full, 1); mbar_init(s_full + 8, 1); mbar_init(p_ready, 128); mbar_init(pv_done, 1); mbar_init(o_free, 128);
+        for (int i = 0; i < 14; ++i) mbar_init(smem_u32(bars + i), 1);
+        mbar_init(p_ready, 128); mbar_init(pv_done, 1); mbar_init(o_free, 128);
         mbar_init_fence();
-        tma_prefetch_desc(&kmap); tma_prefetch_desc(&vmap);
+        tma_prefetch_desc(&qmap); tma_prefetch_desc(&kmap); tma_prefetch_desc(&vmap);
     }
     if (warp == 1) tmem_alloc(smem_u32(tmem_slot), TMEM_COLS);
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
     pdl_trigger();                                       // behind the allocation: a kernel that starts early may want tensor memory too
-    pdl_wait(q);
+    pdl_wait();
     make_plan<KT>(a, plan);
     __syncthreads();
     const uint32_t tmem = *tmem_slot;
@@ -91,155 +171,121 @@ attn_shared_tc_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_con
         const int box = min(a.ps, KT), ops_per_tile = KT / box * HALVES;
         const uint32_t full = is_v ? v_full : k_full, empty = is_v ? v_empty : k_empty, dst0 = is_v ? sV : sK;
         const CUtensorMap* map = is_v ? &vmap : &kmap;
-        bool ok = true;
-        int n = 0;                                           // tiles so far
-        while (ok && walk.next()) {
-            const int* table = walk.table();
-            for (int i = 0; i < walk.tiles && ok; ++i, ++n) {
-                const int s = n & 1, key = walk.key0 + i * KT;
-                if (lane == 0) {
-                    if (n >= 2 && !mbar_wait(empty + 8 * s, ((n >> 1) - 1) & 1)) { atomicExch(error_word, 61); ok = false; }
-                    if (ok) mbar_expect_tx(full + 8 * s, KV_BYTES);
-                }
-                ok = __shfl_sync(0xffffffffu, ok, 0);
-                if (!ok) break;
-                for (int op = lane; op < ops_per_tile; op += 32) {
-                    const int b = op / HALVES, hb = op % HALVES, j = key + b * box;
-                    const int page = j < walk.hi ? table[j / a.ps] : 0;                        // behind the last key: the null page
-                    tma_load_2d(dst0 + s * KV_BYTES + hb * (KT * 128) + b * box * 128, map, hb * 64, (page * a.KV + walk.kvh) * a.ps + j % a.ps, full + 8 * s);
+        const int b = lane / HALVES, hb = lane % HALVES;     // this lane's box (at most 8 boxes of two halves)
+        bool ok = true, more = walk.next();
+        int i = 0, page = 0, before = BQ;                    // the piece's tile; matrix rows of the piece in front
+        const int* table = nullptr;
+        const auto ask = [&]() {                             // for the next tile's page; behind the last key: the null page
+            const int j = walk.key0 + i * KT + b * box;
+            page = lane < ops_per_tile && j < walk.hi ? table[j / a.ps] : 0;
+        };
+        if (more) { table = walk.table(); ask(); }
+        for (int n = 0, piece = 0; more; ++n) {
+            const int s = n & 1;
+            if (!is_v && i == 0) {                           // the piece's queries, once the rows that they take are done with
+                const int rows = walk.rows * Hg, copies = copies_of(1, rows), apart = BQ / copies, off = rows <= 16 && piece & 1 ? 16 : 0;
+                if (piece >= 2) ok = mbar_wait(q_done + 8 * (piece & 1), ((piece >> 1) - 1) & 1);
+                if (ok && piece && (rows > 16 || before > 16)) ok = mbar_wait(q_done + 8 * ((piece - 1) & 1), ((piece - 1) >> 1) & 1);
+                if (!__all_sync(0xffffffffu, ok)) { if (lane == 0) atomicExch(error_word, 60); break; }
+                before = rows;
+                if (lane == 0) mbar_expect_tx(q_full + 8 * (piece & 1), rows * copies * D * 2);
+                __syncwarp();
+                for (int op = lane; op < walk.rows * copies * HALVES; op += 32) {
+                    const int half = op % HALVES, set = op / HALVES % copies, r = op / HALVES / copies;
+                    tma_load_3d(sQ + half * (BQ * 128) + (set * apart + off + r * Hg) * 128, &qmap, half * 64, walk.kvh * Hg, plan.token[walk.row0 + r], q_full + 8 * (piece & 1));
                 }
             }
+            if (lane == 0) {
+                if (n >= 2 && !mbar_wait(empty + 8 * s, ((n >> 1) - 1) & 1)) { atomicExch(error_word, 61); ok = false; }
+                if (ok) mbar_expect_tx(full + 8 * s, KV_BYTES);
+            }
+            ok = __shfl_sync(0xffffffffu, ok, 0);
+            if (!ok) break;
+            if (lane < ops_per_tile)
+                tma_load_2d(dst0 + s * KV_BYTES + hb * (KT * 128) + b * box * 128, map, hb * 64, (page * a.KV + walk.kvh) * a.ps + (walk.key0 + i * KT + b * box) % a.ps, full + 8 * s);
+            if (++i == walk.tiles) {
+                i = 0;
+                ++piece;
+                more = walk.next();
+                if (more) table = walk.table();
+            }
+            if (more) ask();
         }
     } else if (warp == 1) {
         // ---------------- MMA issue
         if (lane == 0) {
             const uint32_t idesc_s = umma_idesc_bf16(BQ, KT, false);      // S[128 x 64]  = Q (K-major) * K^T (K-major)
             const uint32_t idesc_o = umma_idesc_bf16(BQ, D, true);        // O[128 x D]  += P (tensor memory) * V (MN-major)
-            bool ok = true;
-            int n = 0, pieces = 0;
-            auto issue_qk = [&](int m) {
-                const int s = m & 1;
-                if (!mbar_wait(k_full + 8 * s, (m >> 1) & 1)) { atomicExch(error_word, 63); ok = false; return; }
-                tc_fence_after();
+            Walk<KT> ahead(a, plan);                         // the scores' way, up to a tile in front
+            bool more_s = ahead.next(), more_o = walk.next();
+            int m = 0, tile_s = 0, piece_s = 0;              // the next scores: tile, tile of their piece, piece
+            int n = 0, tile_o = 0, piece_o = 0;              // the next weighted sum
+            for (uint32_t spins = 0; more_o; ++spins) {
+                if (spins == SPIN_LIMIT << 4) { atomicExch(error_word, 63); break; }
+                // scores go to the buffer whose weights the sum before last used
+                if (more_s && m <= n + 1 && mbar_test(k_full + 8 * (m & 1), (m >> 1) & 1) && (tile_s || mbar_test(q_full + 8 * (piece_s & 1), (piece_s >> 1) & 1))) {
+                    const int s = m & 1;
+                    tc_fence_after();
 #pragma unroll
-                for (int ks = 0; ks < D / 16; ++ks) {
-                    const uint32_t qa = sQ + (ks / 4) * (BQ * 128) + (ks % 4) * 32, kb = sK + s * KV_BYTES + (ks / 4) * (KT * 128) + (ks % 4) * 32;
-                    umma_ss(tmem + S_COL + 64 * s, umma_desc_sw128(qa, 16, 1024), umma_desc_sw128(kb, 16, 1024), idesc_s, ks != 0);
+                    for (int ks = 0; ks < D / 16; ++ks) {
+                        const uint32_t qa = sQ + (ks / 4) * (BQ * 128) + (ks % 4) * 32, kb = sK + s * KV_BYTES + (ks / 4) * (KT * 128) + (ks % 4) * 32;
+                        umma_ss(tmem + S_COL + 64 * s, umma_desc_sw128(qa, 16, 1024), umma_desc_sw128(kb, 16, 1024), idesc_s, ks != 0);
+                    }
+                    umma_commit(k_empty + 8 * s);              // the keys of this stage are free once these finish
+                    umma_commit(s_full + 8 * s);
+                    ++m;
+                    if (++tile_s == ahead.tiles) {
+                        umma_commit(q_done + 8 * (piece_s & 1));
+                        tile_s = 0;
+                        ++piece_s;
+                        more_s = ahead.next();
+                    }
+                    spins = 0;
                 }
-                umma_commit(k_empty + 8 * s);                  // the keys of this stage are free once these finish
-                umma_commit(s_full + 8 * s);
-            };
-            while (ok && walk.next()) {
-                if (!mbar_wait(q_full, pieces & 1)) { atomicExch(error_word, 64); break; }
-                issue_qk(n);
-                for (int i = 0; i < walk.tiles && ok; ++i, ++n) {
+                if (n < m && mbar_test(p_ready, n & 1) && mbar_test(v_full + 8 * (n & 1), (n >> 1) & 1) && (tile_o || !piece_o || mbar_test(o_free, (piece_o - 1) & 1))) {
                     const int s = n & 1;
-                    if (i + 1 < walk.tiles) issue_qk(n + 1);       // a tile ahead of the softmax, within a piece
-                    if (!ok) break;
-                    if (!mbar_wait(p_ready, n & 1)) { atomicExch(error_word, 65); ok = false; break; }
-                    if (!mbar_wait(v_full + 8 * s, (n >> 1) & 1)) { atomicExch(error_word, 66); ok = false; break; }
-                    if (i == 0 && pieces > 0 && !mbar_wait(o_free, (pieces - 1) & 1)) { atomicExch(error_word, 67); ok = false; break; }
                     tc_fence_after();
 #pragma unroll
                     for (int kk = 0; kk < KT / 16; ++kk)
-                        umma_ts(tmem + O_COL, tmem + S_COL + 64 * s + kk * 8, umma_desc_sw128(sV + s * KV_BYTES + kk * (16 * 128), KT * 128, 1024), idesc_o, (i | kk) != 0);
+                        umma_ts(tmem + O_COL, tmem + S_COL + 64 * s + kk * 8, umma_desc_sw128(sV + s * KV_BYTES + kk * (16 * 128), KT * 128, 1024), idesc_o, (tile_o | kk) != 0);
                     umma_commit(v_empty + 8 * s);
                     umma_commit(pv_done);
+                    ++n;
+                    if (++tile_o == walk.tiles) {
+                        tile_o = 0;
+                        ++piece_o;
+                        more_o = walk.next();
+                    }
+                    spins = 0;
                 }
-                ++pieces;
             }
         }
     } else {
         // ---------------- softmax: thread <-> (row, head) <-> tensor-memory lane
-        const int lg = warp & 3, mine = lg * 32 + lane, tid = threadIdx.x - 64;
+        const int lg = warp & 3, tid = threadIdx.x - 64;
         const uint32_t lane_addr = tmem + ((uint32_t)(lg * 32) << 16);
-        auto bring_queries = [&](const Walk<KT>& w) {          // the piece's queries into swizzled rows of shared memory, eight pieces of 16 bytes of a thread in flight
-            constexpr int C = D / 8, STEP = 128 / C;
-            const int c = tid % C, first = tid / C, n = w.rows * Hg;
-            for (int row0 = first; row0 < n; row0 += 8 * STEP) {
-                uint4 v[8];
-#pragma unroll
-                for (int k = 0; k < 8; ++k) {
-                    const int row = row0 + k * STEP;
-                    if (row < n) v[k] = *reinterpret_cast<const uint4*>(q + (size_t)plan.token[w.row0 + row / Hg] * q_stride + (size_t)(w.kvh * Hg + row % Hg) * D + c * 8);
-                }
-#pragma unroll
-                for (int k = 0; k < 8; ++k) {
-                    const int row = row0 + k * STEP;
-                    if (row < n) *reinterpret_cast<uint4*>(base + (c / 8) * (BQ * 128) + row * 128 + (((c % 8) ^ (row & 7)) << 4)) = v[k];
-                }
-            }
-            asm volatile("fence.proxy.async.shared::cta;\n" ::: "memory");
-            mbar_arrive(q_full);
-        };
-        bool ok = true, more = walk.next();
+        bool ok = true;
         int n = 0;
-        if (more) bring_queries(walk);
-        while (more && ok) {
-            const int rows = walk.rows * Hg, tiles = walk.tiles, key0 = walk.key0, lo = walk.lo, place = walk.place();
-            const bool prefix = walk.prefix, active = lg * 32 < rows;
-            const int hi = walk.hi;
+        for (int piece = 0; ok && walk.next(); ++piece) {
+            const int rows = walk.rows * Hg, tiles = walk.tiles, lo = walk.lo, hi = walk.hi;
+            const int copies = copies_of(1, rows), warps = 4 / copies, copy = lg / warps, col = copy * (KT / copies);
+            const int mine = lg % warps * 32 + lane - (rows <= 16 && piece & 1 ? 16 : 0);      // the row
+            const bool there = mine >= 0 && mine < rows, active = __any_sync(0xffffffffu, there);
             // a prefix's rows see no further than their own length; lanes beyond the rows hold anything
-            const int mine_hi = mine < rows ? min(hi, plan.keys[walk.row0 + mine / Hg]) : hi;
-            float m_ref = -INFINITY, l = 0.f;
+            const int mine_hi = there ? min(hi, plan.keys[walk.row0 + mine / Hg]) : hi;
+            Row row{-INFINITY, 0.f};
             for (int i = 0; i < tiles && ok; ++i, ++n) {
-                const int s = n & 1, key = key0 + i * KT;
+                const int s = n & 1, key = walk.key0 + i * KT;
                 const uint32_t s_addr = lane_addr + S_COL + 64 * s;
                 if (!mbar_wait(s_full + 8 * s, (n >> 1) & 1)) { atomicExch(error_word, 68); ok = false; break; }
                 tc_fence_after();
                 float alpha = 1.f;
                 bool rescale = false;
                 if (active) {
-                    // The scores in two halves of 32, read twice: for the maximum, and for the weights (few registers, little code)
-                    const bool whole = __all_sync(0xffffffffu, key >= lo && key + KT <= mine_hi);
-                    const uint32_t from = (uint32_t)(key - lo), span = (uint32_t)max(mine_hi - lo, 0);      // a key in front of lo wraps around
-                    float mx4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-                    uint32_t r[32];
-#pragma unroll 1
-                    for (int half = 1; half >= 0; --half) {
-                        tmem_ld32(s_addr + 32 * half, r);
-                        tmem_wait_ld();
-                        if (!whole) {
-#pragma unroll
-                            for (int c = 0; c < 32; ++c) r[c] = from + (half * 32 + c) < span ? r[c] : 0xff800000u;       // -inf
-                        }
-#pragma unroll
-                        for (int c = 0; c < 32; c += 8)
-#pragma unroll
-                            for (int e = 0; e < 4; ++e) mx4[e] = max3(mx4[e], __uint_as_float(r[c + 2 * e]), __uint_as_float(r[c + 2 * e + 1]));
-                    }
-                    const float mx = fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3])) * scale_log2;      // scale > 0
-                    if (mx > m_ref + 8.f) {
-                        alpha = m_ref == -INFINITY ? 0.f : fast_exp2(m_ref - mx);
-                        rescale = i > 0 && m_ref != -INFINITY;
-                        m_ref = mx;
-                        l *= alpha;
-                    }
-                    const float off = m_ref == -INFINITY ? 0.f : m_ref;
-                    const float2 scale2 = make_float2(scale_log2, scale_log2), noff2 = make_float2(-off, -off);
-                    float2 sums[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
-#pragma unroll 1
-                    for (int half = 0; half < 2; ++half) {             // r holds the first half
-                        if (half) {
-                            tmem_ld32(s_addr + 32, r);
-                            tmem_wait_ld();
-                            if (!whole) {
-#pragma unroll
-                                for (int c = 0; c < 32; ++c) r[c] = from + (32 + c) < span ? r[c] : 0xff800000u;
-                            }
-                        }
-                        uint32_t pk[16];
-#pragma unroll
-                        for (int c = 0; c < 16; ++c) {
-                            const float2 arg = __ffma2_rn(make_float2(__uint_as_float(r[2 * c]), __uint_as_float(r[2 * c + 1])), scale2, noff2);
-                            const float2 p = make_float2(fast_exp2(arg.x), fast_exp2(arg.y));
-                            sums[c & 1] = __fadd2_rn(sums[c & 1], p);
-                            pk[c] = pack_bf16(p.x, p.y);
-                        }
-                        tmem_st16(s_addr + 16 * half, pk);             // P takes the place of the first scores
-                    }
-                    const float2 s01 = __fadd2_rn(sums[0], sums[1]);
-                    l += s01.x + s01.y;
+                    const bool whole = __all_sync(0xffffffffu, key + col >= lo && key + col + KT / copies <= mine_hi);
+                    const uint32_t from = (uint32_t)(key + col - lo), span = (uint32_t)max(mine_hi - lo, 0);      // a key in front of lo wraps around
+                    if (copies == 4) rescale = weights<16>(s_addr, col, 1, whole, from, span, scale_log2, i == 0, row, alpha);
+                    else rescale = weights<32>(s_addr, col, 2 / copies, whole, from, span, scale_log2, i == 0, row, alpha);
                 }
                 if (key < lo || key + KT > hi) {
                     // Values in front of the piece's first or behind its last key may be anything (a page's unused part), and 0 * inf is no 0
@@ -270,26 +316,23 @@ attn_shared_tc_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_con
                 mbar_arrive(p_ready);
             }
             if (!ok) break;
-            // the last tile's scores are there, so nothing reads this piece's queries any more
-            more = walk.next();
-            if (more) bring_queries(walk);
             if (!mbar_wait(pv_done, (n - 1) & 1)) { atomicExch(error_word, 70); break; }
             tc_fence_after();
             if (active) {
-                const int rows_of = prefix ? a.slot_rows : Hg;
-                float4* to = reinterpret_cast<float4*>(prefix ? a.o_prefix : a.o_tail) + (size_t)place * (D / 4) * rows_of + mine;
+                const int rows_of = walk.prefix ? a.slot_rows : a.tail_rows, at = copy * rows + mine;
+                float4* to = reinterpret_cast<float4*>(walk.prefix ? a.o_prefix : a.o_tail) + (size_t)walk.place() * (D / 4) * rows_of + at;
 #pragma unroll 1
                 for (int c = 0; c < D / 32; ++c) {
                     uint32_t o[32];
                     tmem_ld32(lane_addr + O_COL + c * 32, o);
                     tmem_wait_ld();
-                    if (mine < rows) {
+                    if (there) {
 #pragma unroll
                         for (int v4 = 0; v4 < 8; ++v4)
                             to[(size_t)(c * 8 + v4) * rows_of] = make_float4(__uint_as_float(o[4 * v4]), __uint_as_float(o[4 * v4 + 1]), __uint_as_float(o[4 * v4 + 2]), __uint_as_float(o[4 * v4 + 3]));
                     }
                 }
-                if (mine < rows) (prefix ? a.ml_prefix : a.ml_tail)[(size_t)place * rows_of + mine] = make_float2(m_ref, l);
+                if (there) (walk.prefix ? a.ml_prefix : a.ml_tail)[(size_t)walk.place() * rows_of + at] = make_float2(row.m, row.l);
             }
             tc_fence_before();
             mbar_arrive(o_free);
@@ -316,43 +359,58 @@ bool cache_map(const void* cache, long long rows, int D, int box, CUtensorMap* o
     return true;
 }
 
+// The queries [tokens, heads, D], rows of tokens `stride` elements apart, in boxes of a key head's query heads x 64
+bool query_map(const void* q, int tokens, int H, int D, long long stride, int heads, CUtensorMap* out) {
+    auto fn = sm100_host::encoder();
+    if (!fn) return false;
+    const cuuint64_t dims[3] = {(cuuint64_t)D, (cuuint64_t)H, (cuuint64_t)tokens}, strides[2] = {(cuuint64_t)D * 2, (cuuint64_t)stride * 2};
+    const cuuint32_t box[3] = {64, (cuuint32_t)heads, 1}, one[3] = {1, 1, 1};
+    return fn(out, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, const_cast<void*>(q), dims, strides, box, one, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+              CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
 bool fits(int R, int G, int H, int KV, int D, int ps) {
     return R > 0 && G >= 0 && R + G <= MAX_ENTITIES && KV > 0 && H % KV == 0 && H / KV <= BQ && (D == 64 || D == 128) && ps % 8 == 0 &&
            (ps <= KT ? KT % ps == 0 : ps % KT == 0) && KV <= 65535;
 }
 int tile_rows_of(int H, int KV) { return BQ / (H / KV); }
 int row_tiles_of(int H, int KV, int most) { const int t = tile_rows_of(H, KV); return most > 1 ? (most + t - 1) / t : 1; }
-int slot_rows_of(int H, int KV, int most) { const int t = tile_rows_of(H, KV); return (most < t ? (most > 1 ? most : 1) : t) * (H / KV); }
+int slot_rows_of(int H, int KV, int most) {          // with the copies of any number of rows up to the largest tile's
+    const int t = tile_rows_of(H, KV), rows = (most < t ? (most > 1 ? most : 1) : t) * (H / KV);
+    return rows <= BQ / 4 ? 4 * rows : BQ;
+}
+int tail_rows_of(int H, int KV) { return copies_of(1, H / KV) * (H / KV); }
 
 }  // namespace
 
 // Bytes of the work space of a call; -2: sizes that this kernel does not take.  most: rows of the largest group.
 MI_EXPORT long long mi_attn_shared_tc_bytes(int R, int G, int most, int H, int KV, int D, int ps) {
     if (!fits(R, G, H, KV, D, ps)) return -2;
-    return scratch(R, G, H, KV, D, row_tiles_of(H, KV, most), slot_rows_of(H, KV, most), 2 * device_sms()).bytes;
+    return scratch(R, G, KV, D, row_tiles_of(H, KV, most), slot_rows_of(H, KV, most), tail_rows_of(H, KV), 2 * device_sms()).bytes;
 }
 
-// q, out bfloat16 ([tokens, H D], rows of q q_stride apart); caches [pages, KV, ps, D] with cache_rows = pages KV ps; decode_segs int32 [R] (the entries, one token
+// q, out bfloat16 ([tokens, H D], rows of q q_stride apart); caches [pages, KV, ps, D] with cache_rows = pages KV ps; decode_segs int32 [R] (which of the `entries` feed one token
 // each), shared_start int32 [G + 1] over them, shared_len int32 [G]; block_table rows table_stride apart (entry i reads row table_rows[i], or i).
-MI_EXPORT int mi_attn_shared_tc(const void* q, int q_stride, const void* k_cache, const void* v_cache, long long cache_rows, void* out, const int* decode_segs, int R,
-                                const int* seg_q_start, const int* seg_kv_len, const int* block_table, const int* table_rows, int table_stride,
+MI_EXPORT int mi_attn_shared_tc(const void* q, int q_stride, int tokens, const void* k_cache, const void* v_cache, long long cache_rows, void* out, const int* decode_segs, int R,
+                                const int* seg_q_start, const int* seg_kv_len, int entries, const int* block_table, const int* table_rows, int table_stride,
                                 const int* shared_start, const int* shared_len, int G, int most, int H, int KV, int D, int ps, float scale, void* work,
                                 int* error_word, cudaStream_t stream) {
     if (R == 0) return 0;
-    if (!fits(R, G, H, KV, D, ps) || q_stride % 8 || cache_rows > 0x7fffffff || (((uintptr_t)q | (uintptr_t)k_cache | (uintptr_t)v_cache | (uintptr_t)work) % 16)) return -2;
-    CUtensorMap kmap, vmap;
+    if (!fits(R, G, H, KV, D, ps) || entries < 1 || tokens < 1 || q_stride % 8 || cache_rows > 0x7fffffff || (((uintptr_t)q | (uintptr_t)k_cache | (uintptr_t)v_cache | (uintptr_t)work) % 16)) return -2;
+    CUtensorMap qmap, kmap, vmap;
+    if (!query_map(q, tokens, H, D, q_stride, H / KV, &qmap)) return -5;
     if (!cache_map(k_cache, cache_rows, D, ps < KT ? ps : KT, &kmap) || !cache_map(v_cache, cache_rows, D, ps < KT ? ps : KT, &vmap)) return -5;
     const int blocks = 2 * device_sms();
-    Args a{decode_segs, seg_q_start, seg_kv_len, block_table, table_rows, shared_start, shared_len, R, G, most > 1 ? most : 1, table_stride, H, KV, ps,
-           row_tiles_of(H, KV, most), tile_rows_of(H, KV), slot_rows_of(H, KV, most)};
-    place_scratch(a, scratch(R, G, H, KV, D, a.row_tiles, a.slot_rows, blocks), work);
-    const auto bytes = [&](int ints) { return (size_t)BQ * D * 2 + 4 * (size_t)KT * D * 2 + 16 * 8 + (size_t)ints * 4 + 1024; };
+    Args a{decode_segs, seg_q_start, seg_kv_len, block_table, table_rows, shared_start, shared_len, R, G, entries, most > 1 ? most : 1, table_stride, H, KV, ps,
+           row_tiles_of(H, KV, most), tile_rows_of(H, KV), 1, slot_rows_of(H, KV, most), tail_rows_of(H, KV)};
+    place_scratch(a, scratch(R, G, KV, D, a.row_tiles, a.slot_rows, a.tail_rows, blocks), work);
+    const auto bytes = [&](int ints) { return (size_t)BQ * D * 2 + 4 * (size_t)KT * D * 2 + 18 * 8 + (size_t)ints * 4 + 1024; };
     const size_t smem = bytes(plan_ints(G, R)), most_smem = bytes(6 * MAX_ENTITIES + 1);
     const float scale_log2 = scale * LOG2E;
 #define LAUNCH(DD) do { \
-        cudaError_t e = cudaFuncSetAttribute(attn_shared_tc_kernel<DD>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)most_smem); \
-        if (e == cudaSuccess) e = launch_pdl(attn_shared_tc_kernel<DD>, dim3(blocks), dim3(THREADS), smem, stream, kmap, vmap, a, (const __nv_bfloat16*)q, \
-                                             (long long)q_stride, scale_log2, error_word); \
+        static unsigned long long done = 0; \
+        cudaError_t e = allow_shared(attn_shared_tc_kernel<DD>, (int)most_smem, done); \
+        if (e == cudaSuccess) e = launch_pdl(attn_shared_tc_kernel<DD>, dim3(blocks), dim3(THREADS), smem, stream, qmap, kmap, vmap, a, scale_log2, error_word); \
         if (e == cudaSuccess) e = launch_pdl(merge_kernel<__nv_bfloat16, DD>, dim3(R, KV), dim3(128 * MERGE_PARTS), 0, stream, a, (__nv_bfloat16*)out); \
         return (int)e; \
     } while (0)

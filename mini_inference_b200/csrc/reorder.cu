@@ -89,8 +89,10 @@ MI_EXPORT int mi_reorder_rows(const long long* tensors, int count, const int* ro
     if (count < 0 || groups < 0 || groups > 65535 || num_rows < 0 || most < 0 || most > MOST_ROWS) return -2;
     if (!count || !groups || !num_rows || !most) return 0;
     const size_t smem = (size_t)most * CHUNK;
-    const cudaError_t fit = cudaFuncSetAttribute(reorder_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, MOST_ROWS * CHUNK);
-    if (fit != cudaSuccess) return -1000 - (int)fit;
+    if (smem > 40 * 1024) {                          // (with the lists; up to 48 KB need no leave)
+        const cudaError_t fit = cudaFuncSetAttribute(reorder_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, MOST_ROWS * CHUNK);
+        if (fit != cudaSuccess) return -1000 - (int)fit;
+    }
     int launches = 0;
     for (int first = 0; first < count;) {
         RowTensors all = {};

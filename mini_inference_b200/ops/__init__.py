@@ -10,7 +10,6 @@ of float32 sums whether they run as multiply-adds or as bfloat16 parts on the te
 from __future__ import annotations
 
 import array
-import contextlib
 import ctypes
 import math
 import os
@@ -66,7 +65,6 @@ def load_calls():
 
 
 _CODES = {torch.float32: 0, torch.bfloat16: 1}
-_NOTHING = contextlib.nullcontext()
 
 
 def _code(dtype):
@@ -76,6 +74,7 @@ def _code(dtype):
         raise TypeError(f"dtype {dtype} is not supported by the kernels (float32, bfloat16)") from None
 
 
+_current_device = getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.current_device
 _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda device_index: torch.cuda.current_stream(device_index).cuda_stream)
 
 
@@ -707,15 +706,17 @@ class CudaOps:
         raise AssertionError(f"{what}: refused without a reason")
 
     def _shared_or_alone(self, q, k_cache, v_cache, meta, H, KV, D, scale):
-        with self._current():
-            size = self._shared_bytes(q, k_cache, v_cache, meta, H, KV, D)
-            if size <= 0:
-                alone = types.SimpleNamespace(prefill_tiles=meta.decode_segs[:0].view(0, 2), tile=self.prefill_tile, max_kv_len=meta.max_kv_len, max_pages=meta.max_pages,
-                                              page_size=meta.page_size, block_table=meta.block_table, table_rows=getattr(meta, "table_rows", None), shared_start=None,
-                                              decode_segs=meta.decode_segs, seg_q_start=meta.seg_q_start, seg_kv_len=meta.seg_kv_len)
-                return self.paged_attention(q, k_cache, v_cache, alone, H, KV, D, scale, None)
-            out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-            self._shared_decode(q, k_cache, v_cache, out, meta, H, KV, D, scale, size)
+        if self._elsewhere():
+            with torch.cuda.device(self._device_index):
+                return self._shared_or_alone(q, k_cache, v_cache, meta, H, KV, D, scale)
+        size = self._shared_bytes(q, k_cache, v_cache, meta, H, KV, D)
+        if size <= 0:
+            alone = types.SimpleNamespace(prefill_tiles=meta.decode_segs[:0].view(0, 2), tile=self.prefill_tile, max_kv_len=meta.max_kv_len, max_pages=meta.max_pages,
+                                          page_size=meta.page_size, block_table=meta.block_table, table_rows=getattr(meta, "table_rows", None), shared_start=None,
+                                          decode_segs=meta.decode_segs, seg_q_start=meta.seg_q_start, seg_kv_len=meta.seg_kv_len)
+            return self.paged_attention(q, k_cache, v_cache, alone, H, KV, D, scale, None)
+        out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+        self._shared_decode(q, k_cache, v_cache, out, meta, H, KV, D, scale, size)
         return out
 
     def _shared_bytes(self, q, k_cache, v_cache, meta, H, KV, D):
@@ -727,10 +728,10 @@ class CudaOps:
 
     def _shared_decode(self, q, k_cache, v_cache, out, meta, H, KV, D, scale, size):
         work = torch.empty(size, dtype=torch.uint8, device=q.device)
-        rows = (out, meta.decode_segs, meta.decode_segs.shape[0], meta.seg_q_start, meta.seg_kv_len, meta.block_table, getattr(meta, "table_rows", None), meta.max_pages,
+        rows = (out, meta.decode_segs, meta.decode_segs.shape[0], meta.seg_q_start, meta.seg_kv_len, meta.seg_kv_len.shape[0], meta.block_table, getattr(meta, "table_rows", None), meta.max_pages,
                 meta.shared_start, meta.shared_len, meta.shared_len.shape[0], meta.max_shared_rows, H, KV, D, meta.page_size, scale, work)
         if q.dtype is torch.bfloat16:
-            _check(self.lib.mi_attn_shared_tc(q, q.stride(0), k_cache, v_cache, k_cache.shape[0] * KV * meta.page_size, *rows, self._stream_error, self._stream()),
+            _check(self.lib.mi_attn_shared_tc(q, q.stride(0), q.shape[0], k_cache, v_cache, k_cache.shape[0] * KV * meta.page_size, *rows, self._stream_error, self._stream()),
                    "attn_shared_tc")
         else:
             _check(self.lib.mi_attn_shared_f32(q, q.stride(0), k_cache, v_cache, *rows, self._stream()), "attn_shared_f32")
@@ -1800,9 +1801,9 @@ class CudaOps:
             if not t.is_contiguous():
                 raise ValueError(f"{what}: {name} is not contiguous")
 
-    def _current(self):
-        """The device made current for a launch, where another one is."""
-        return _NOTHING if torch.cuda.current_device() == self._device_index else torch.cuda.device(self._device_index)
+    def _elsewhere(self):
+        """Whether another device is the current one: a launch needs this one to be (torch.cuda.device(self._device_index))."""
+        return _current_device() != self._device_index
 
     def beam_select(self, logits, scores, group_start, num):
         """A beam search step's candidates.  logits float32 [R, V] (rows may be strided), scores float32 [R]: a row per beam and the sum of
@@ -1819,17 +1820,19 @@ class CudaOps:
         (R, V), G, ld = logits.shape, group_start.shape[0] - 1, logits.stride(0)
         if V < 1 or (V > 1 and logits.stride(1) != 1) or (R > 1 and ld < V):
             raise ValueError(f"beam_select: logits of shape {tuple(logits.shape)} with strides {logits.stride()} (a row's logits lie side by side)")
+        if self._elsewhere():
+            with torch.cuda.device(here):
+                return self.beam_select(logits, scores, group_start, num)
         dev = logits.device
         values = torch.empty((G, num), dtype=torch.float32, device=dev)
-        rows, tokens = torch.empty((G, num), dtype=torch.int32, device=dev), torch.empty((G, num), dtype=torch.int32, device=dev)
-        with self._current():
-            n = self.lib.mi_beam_select_bytes(R, V, num)
-            if n < 0:
-                _check(n, "beam_select")
-            work = torch.empty(n, dtype=torch.uint8, device=dev)
-            _check(self.lib.mi_beam_select(logits, ld if R > 1 else V, R, V, scores, group_start, G, num, values, rows, tokens, work, self._stream()), "beam_select")
+        chosen = torch.empty((2, G, num), dtype=torch.int32, device=dev)
+        n = self.lib.mi_beam_select_bytes(R, V, num)
+        if n < 0:
+            _check(n, "beam_select")
+        work = torch.empty(n, dtype=torch.uint8, device=dev)
+        _check(self.lib.mi_beam_select(logits, ld if R > 1 else V, R, V, scores, group_start, G, num, values, chosen, work, self._stream()), "beam_select")
         self.launches += (2 if R else 1) if G else 0
-        return values, rows, tokens
+        return values, *chosen.unbind()
 
     def _refuse_select(self, logits, scores, group_start, num):
         """Raises what is wrong with a call of beam_select."""
@@ -1872,12 +1875,15 @@ class CudaOps:
             places.extend((t.data_ptr(), lead, n * stride, n, stride, row))
         if not rows.get_device() == parents.get_device() == group_start.get_device() == here or any(t.get_device() != here for t in tensors):
             self._here("reorder_rows", rows=rows, parents=parents, group_start=group_start, **{f"tensor {i}": t for i, t in enumerate(tensors)})
-        if tensors:
-            with self._current():
-                done = self.lib.mi_reorder_rows(places.buffer_info()[0], len(tensors), rows, parents, group_start, group_start.shape[0] - 1, rows.shape[0], most, self._stream())
-            if done < 0:
-                _check(done if done > -1000 else -1000 - done, "reorder_rows")
-            self.launches += done
+        if not tensors:
+            return
+        if self._elsewhere():
+            with torch.cuda.device(here):
+                return self.reorder_rows(tensors, rows, parents, group_start, most, dim)
+        done = self.lib.mi_reorder_rows(places.buffer_info()[0], len(tensors), rows, parents, group_start, group_start.shape[0] - 1, rows.shape[0], most, self._stream())
+        if done < 0:
+            _check(done if done > -1000 else -1000 - done, "reorder_rows")
+        self.launches += done
 
 
 _OPS = {}
