@@ -165,18 +165,21 @@ struct Walk {
             if (tiles > 0) return true;
         }
     }
-    __device__ __forceinline__ const int* table() const {
+    __device__ __forceinline__ int table_row() const {
         int holds = who;
         if (prefix) { holds = p.source[who]; if (holds >= p.start[who] + p.rows[who]) holds = p.start[who]; }      // nobody has them all
-        return a.block_table + (size_t)p.table[holds] * a.table_stride;
+        return p.table[holds];
     }
     __device__ __forceinline__ int place() const { return (prefix ? (who * a.KV + kvh) * a.row_tiles + row_tile : who * a.KV + kvh) + (int)blockIdx.x; }
 };
 
+// A piece as one warp of a block writes it down for the others (finding it costs a thousand clocks)
+struct __align__(16) Piece { int prefix, who, kvh, row0, rows, tiles, lo, hi, key0, place, table, spare; };
+
 // out[token of row r, heads of key head] from the row's pieces: a block per (row, key head), as many heads at a time as fill 128 threads with four columns each
 // (neighbouring heads in neighbouring threads).  A warp per head makes the weights of all pieces, then MERGE_PARTS groups of 128 threads take every
 // MERGE_PARTS-th piece, their rows read without waiting for one another, and are added up in the groups' order.
-constexpr int MERGE_PARTS = 4, MERGE_PIECES = 512;   // pieces whose weights are made at a time
+constexpr int MERGE_PARTS = 2, MERGE_PIECES = 512;   // pieces whose weights are made at a time
 template <typename T, int D>
 __global__ void __launch_bounds__(128 * MERGE_PARTS) merge_kernel(const __grid_constant__ Args a, T* __restrict__ out) {
     constexpr int HEADS = 512 / D;
@@ -209,6 +212,16 @@ __global__ void __launch_bounds__(128 * MERGE_PARTS) merge_kernel(const __grid_c
         const int row_p = (rec.prefix_row & 0xffff) + h0, row_t = h0;
         float m = -INFINITY, l = 0.f;                // of this warp's head
         float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+        const auto rows_of = [&](int i) {            // this thread's columns of piece i
+            if (i < n_p) return reinterpret_cast<const float4*>(a.o_prefix) + ((at_p + (i >> shift_p)) * (D / 4) + c) * a.slot_rows + (i & (copies_p - 1)) * rows_p + row_p + h;
+            i -= n_p;
+            return reinterpret_cast<const float4*>(a.o_tail) + ((at_t + (i >> shift_t)) * (D / 4) + c) * a.tail_rows + (i & (copies_t - 1)) * Hg + row_t + h;
+        };
+        constexpr int EARLY = 8;                     // pieces of a thread that are asked for before their weights are there
+        float4 early[EARLY];
+#pragma unroll
+        for (int k = 0; k < EARLY; ++k)
+            if (mine && part + k * MERGE_PARTS < n) early[k] = *rows_of(part + k * MERGE_PARTS);
         for (int i0 = 0; i0 < max(n, 1); i0 += MERGE_PIECES) {
             const int now = min(MERGE_PIECES, n - i0);
             if (warp < heads) {
@@ -242,15 +255,16 @@ __global__ void __launch_bounds__(128 * MERGE_PARTS) merge_kernel(const __grid_c
                     o.x = w == 0.f ? o.x : fmaf(v.x, w, o.x); o.y = w == 0.f ? o.y : fmaf(v.y, w, o.y);
                     o.z = w == 0.f ? o.z : fmaf(v.z, w, o.z); o.w = w == 0.f ? o.w : fmaf(v.w, w, o.w);
                 };
-                const float4* p = reinterpret_cast<const float4*>(a.o_prefix) + (at_p * (D / 4) + c) * a.slot_rows + row_p + h;
-                const float4* q = reinterpret_cast<const float4*>(a.o_tail) + (at_t * (D / 4) + c) * a.tail_rows + row_t + h;
-                const size_t step_p = (size_t)(D / 4) * a.slot_rows, step_q = (size_t)(D / 4) * a.tail_rows;
                 int i = i0 + part;
-                const int end = i0 + now, end_p = min(n_p, end);
+                const int end = i0 + now;
+                if (i0 == 0) {
+#pragma unroll
+                    for (int k = 0; k < EARLY; ++k)
+                        if (part + k * MERGE_PARTS < now) add(early[k], weight[(part + k * MERGE_PARTS) * HEADS + h]);
+                    i += EARLY * MERGE_PARTS;
+                }
 #pragma unroll 4
-                for (; i < end_p; i += MERGE_PARTS) add(p[(i >> shift_p) * step_p + (i & (copies_p - 1)) * rows_p], weight[(i - i0) * HEADS + h]);
-#pragma unroll 2
-                for (; i < end; i += MERGE_PARTS) add(q[((i - n_p) >> shift_t) * step_q + ((i - n_p) & (copies_t - 1)) * Hg], weight[(i - i0) * HEADS + h]);
+                for (; i < end; i += MERGE_PARTS) add(*rows_of(i), weight[(i - i0) * HEADS + h]);
             }
             __syncthreads();
         }

@@ -43,7 +43,7 @@ __global__ void __launch_bounds__(THREADS, 2) attn_shared_f32_kernel(const __gri
     auto load_next = [&](int stage) {                // the line's next tile, if there is one
         if (ahead_tile == ahead_tiles) {
             ahead_tile = ahead_tiles = 0;
-            if (ahead.next()) { ahead_tiles = ahead.tiles; table = ahead.table(); }
+            if (ahead.next()) { ahead_tiles = ahead.tiles; table = a.block_table + (size_t)ahead.table_row() * a.table_stride; }
         }
         if (ahead_tile < ahead_tiles) {
             const int key = ahead.key0 + ahead_tile++ * KT;

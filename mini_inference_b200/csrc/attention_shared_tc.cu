@@ -5,14 +5,15 @@
 // of one key head, 128 / (H / KV) rows; a tail has the H / KV heads of its row.  Lanes beyond them hold whatever was there and write nothing.
 //
 // One block is seven warps, two blocks an SM; a block walks its tiles of 64 keys through all its pieces without a stop:
-//   warp 0     queries (TMA, a box of heads per row) and key tiles (TMA, box by box of the page table's rows) into a ring of two, 128-byte swizzle; runs
-//              ahead over the end of a piece, and asks the page table for a tile while the one before waits for its place
+//   warp 0     finds the block's pieces and writes them down for the others; key tiles (TMA, box by box of the page table's rows) into a ring of two, 128-byte
+//              swizzle, and each piece's queries (a box of heads per row); runs ahead over the end of a piece, and asks the page table for a tile while the one
+//              before waits for its place
 //   warp 6     value tiles, the same way
 //   warp 1     one thread issues S = Q K^T (scores in one of two 64-column buffers of tensor memory) up to a tile ahead, over the end of a piece too, and
 //              O += P V, whichever has its operands first
 //   warps 2-5  a matrix row a thread: mask, running maximum and sum (float32, base 2; the exponent's offset is kept until the maximum has grown by 2^8),
 //              weights as bfloat16 back to tensor memory; values that no row sees are cleared in shared memory (what lies in a page's unused part may be
-//              anything, and 0 * inf is no 0).  At the end of a piece they write its O, maximum and sum.
+//              anything, and 0 * inf is no 0; whole boxes behind the last key come as zeros).  At the end of a piece they write its O, maximum and sum.
 // A warp reaches 32 rows of tensor memory, so with few rows one warp would make all weights while three wait (64 exponentials a thread are 512 clocks).
 // Up to 32 rows therefore stand in the tile four times, up to 64 twice, and each copy's warps take their own part of the 64 columns, the others' weights
 // being 0: a copy is a piece of its own with its own maximum and sum, so the warps need not agree on anything, and the merge adds copies like pieces.
@@ -32,7 +33,7 @@ using namespace mi::shared_attention;
 
 namespace {
 
-constexpr int BQ = 128, KT = 64, THREADS = 224;
+constexpr int BQ = 128, KT = 64, THREADS = 224, PIECES = 8;
 constexpr float LOG2E = 1.4426950408889634f;
 
 __device__ __forceinline__ float max3(float a, float b, float c) {      // one instruction on this architecture
@@ -139,18 +140,21 @@ attn_shared_tc_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_con
     unsigned char* base = (unsigned char*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
     // [Q][K0][K1][V0][V1][barriers][plan]
     uint64_t* bars = reinterpret_cast<uint64_t*>(base + Q_BYTES + 4 * KV_BYTES);
-    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 17);
-    const Plan plan(reinterpret_cast<int*>(bars + 18), a.G, a.R);
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 25);
+    Piece* pieces = reinterpret_cast<Piece*>(bars + 26);                // the last PIECES pieces
+    const Plan plan(reinterpret_cast<int*>(pieces + PIECES), a.G, a.R);
     const uint32_t sQ = smem_u32(base), sK = sQ + Q_BYTES, sV = sK + 2 * KV_BYTES;
     // pairs: of tiles or pieces in turn
     const uint32_t q_full = smem_u32(bars), q_done = smem_u32(bars + 2), k_full = smem_u32(bars + 4), k_empty = smem_u32(bars + 6), s_full = smem_u32(bars + 8),
-                   v_full = smem_u32(bars + 10), v_empty = smem_u32(bars + 12), p_ready = smem_u32(bars + 14), pv_done = smem_u32(bars + 15), o_free = smem_u32(bars + 16);
+                   v_full = smem_u32(bars + 10), v_empty = smem_u32(bars + 12), p_ready = smem_u32(bars + 14), pv_done = smem_u32(bars + 15), o_free = smem_u32(bars + 16),
+                   found = smem_u32(bars + 17);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int Hg = a.H / a.KV;
 
     if (threadIdx.x == 0) {
         for (int i = 0; i < 14; ++i) mbar_init(smem_u32(bars + i), 1);
         mbar_init(p_ready, 128); mbar_init(pv_done, 1); mbar_init(o_free, 128);
+        for (int i = 0; i < PIECES; ++i) mbar_init(found + 8 * i, 1);
         mbar_init_fence();
         tma_prefetch_desc(&qmap); tma_prefetch_desc(&kmap); tma_prefetch_desc(&vmap);
     }
@@ -163,51 +167,77 @@ attn_shared_tc_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_con
     make_plan<KT>(a, plan);
     __syncthreads();
     const uint32_t tmem = *tmem_slot;
-    Walk<KT> walk(a, plan);
+    // Piece i, once it is found; false behind the last one (or with a wait that ran out).  Warp 0 is at most four pieces in front of all who read them: it waits
+    // for the queries' rows of the piece before last, whose scores wait for the weights of the tile before last.
+    const auto piece_at = [&](int i, Piece& piece) {
+        if (!mbar_wait(found + 8 * (i % PIECES), (i / PIECES) & 1)) { atomicExch(error_word, 59); return false; }
+        const int4* from = reinterpret_cast<const int4*>(pieces + i % PIECES);
+        int4* to = reinterpret_cast<int4*>(&piece);
+        to[0] = from[0]; to[1] = from[1]; to[2] = from[2];
+        return piece.tiles > 0;
+    };
+    Piece at;
 
     if (warp == 0 || warp == 6) {
         // ---------------- loads.  Lane 0 owns the barriers; the boxes of a tile are issued by one lane each.
         const bool is_v = warp == 6;
-        const int box = min(a.ps, KT), ops_per_tile = KT / box * HALVES;
+        const int box = min(a.ps, KT), ops_per_tile = KT / box * HALVES, b = lane / HALVES, hb = lane % HALVES;       // this lane's box (at most 8) and half
         const uint32_t full = is_v ? v_full : k_full, empty = is_v ? v_empty : k_empty, dst0 = is_v ? sV : sK;
         const CUtensorMap* map = is_v ? &vmap : &kmap;
-        const int b = lane / HALVES, hb = lane % HALVES;     // this lane's box (at most 8 boxes of two halves)
-        bool ok = true, more = walk.next();
+        Walk<KT> walk(a, plan);
+        const auto next = [&](int piece) {
+            if (is_v) return piece_at(piece, at);
+            const bool more = walk.next();
+            if (more) {
+                at.prefix = walk.prefix; at.who = walk.who; at.kvh = walk.kvh; at.row0 = walk.row0; at.rows = walk.rows; at.tiles = walk.tiles; at.lo = walk.lo; at.hi = walk.hi;
+                at.key0 = walk.key0; at.place = walk.place(); at.table = walk.table_row();
+            } else at.tiles = 0;
+            if (lane == 0) {
+                pieces[piece % PIECES] = at;
+                mbar_arrive(found + 8 * (piece % PIECES));
+            }
+            return more;
+        };
+        bool ok = true, more = next(0);
         int i = 0, page = 0, before = BQ;                    // the piece's tile; matrix rows of the piece in front
         const int* table = nullptr;
-        const auto ask = [&]() {                             // for the next tile's page; behind the last key: the null page
-            const int j = walk.key0 + i * KT + b * box;
-            page = lane < ops_per_tile && j < walk.hi ? table[j / a.ps] : 0;
+        const auto ask = [&]() {                             // for the next tile's page; behind the last key: none
+            const int j = at.key0 + i * KT + b * box;
+            page = lane < ops_per_tile && j < at.hi ? table[j / a.ps] : -1;
         };
-        if (more) { table = walk.table(); ask(); }
+        if (more) { table = a.block_table + (size_t)at.table * a.table_stride; ask(); }
         for (int n = 0, piece = 0; more; ++n) {
             const int s = n & 1;
-            if (!is_v && i == 0) {                           // the piece's queries, once the rows that they take are done with
-                const int rows = walk.rows * Hg, copies = copies_of(1, rows), apart = BQ / copies, off = rows <= 16 && piece & 1 ? 16 : 0;
-                if (piece >= 2) ok = mbar_wait(q_done + 8 * (piece & 1), ((piece >> 1) - 1) & 1);
-                if (ok && piece && (rows > 16 || before > 16)) ok = mbar_wait(q_done + 8 * ((piece - 1) & 1), ((piece - 1) >> 1) & 1);
-                if (!__all_sync(0xffffffffu, ok)) { if (lane == 0) atomicExch(error_word, 60); break; }
-                before = rows;
-                if (lane == 0) mbar_expect_tx(q_full + 8 * (piece & 1), rows * copies * D * 2);
-                __syncwarp();
-                for (int op = lane; op < walk.rows * copies * HALVES; op += 32) {
-                    const int half = op % HALVES, set = op / HALVES % copies, r = op / HALVES / copies;
-                    tma_load_3d(sQ + half * (BQ * 128) + (set * apart + off + r * Hg) * 128, &qmap, half * 64, walk.kvh * Hg, plan.token[walk.row0 + r], q_full + 8 * (piece & 1));
-                }
-            }
             if (lane == 0) {
                 if (n >= 2 && !mbar_wait(empty + 8 * s, ((n >> 1) - 1) & 1)) { atomicExch(error_word, 61); ok = false; }
                 if (ok) mbar_expect_tx(full + 8 * s, KV_BYTES);
             }
             ok = __shfl_sync(0xffffffffu, ok, 0);
             if (!ok) break;
-            if (lane < ops_per_tile)
-                tma_load_2d(dst0 + s * KV_BYTES + hb * (KT * 128) + b * box * 128, map, hb * 64, (page * a.KV + walk.kvh) * a.ps + (walk.key0 + i * KT + b * box) % a.ps, full + 8 * s);
-            if (++i == walk.tiles) {
+            if (lane < ops_per_tile) {
+                // no page: a row in front of the first one, which comes as zeros
+                const int y = page < 0 ? -box : (page * a.KV + at.kvh) * a.ps + (at.key0 + i * KT + b * box) % a.ps;
+                tma_load_2d(dst0 + s * KV_BYTES + hb * (KT * 128) + b * box * 128, map, hb * 64, y, full + 8 * s);
+            }
+            if (!is_v && i == 0) {                           // the piece's queries, once the rows that they take are done with
+                const int rows = at.rows * Hg, copies = copies_of(1, rows), apart = BQ / copies, off = rows <= 16 && piece & 1 ? 16 : 0;
+                if (piece >= 2) ok = mbar_wait(q_done + 8 * (piece & 1), ((piece >> 1) - 1) & 1);
+                if (ok && piece && (rows > 16 || before > 16)) ok = mbar_wait(q_done + 8 * ((piece - 1) & 1), ((piece - 1) >> 1) & 1);
+                if (!__all_sync(0xffffffffu, ok)) { if (lane == 0) atomicExch(error_word, 60); break; }
+                before = rows;
+                if (lane == 0) mbar_expect_tx(q_full + 8 * (piece & 1), rows * copies * D * 2);
+                __syncwarp();
+                for (int op = lane; op < at.rows * copies * HALVES; op += 32) {
+                    const int half = op % HALVES, set = op / HALVES & (copies - 1), r = op / HALVES / copies;
+                    tma_load_3d(sQ + half * (BQ * 128) + (set * apart + off + r * Hg) * 128, &qmap, half * 64, at.kvh * Hg, plan.token[at.row0 + r], q_full + 8 * (piece & 1));
+                }
+            }
+            if (++i == at.tiles) {
                 i = 0;
                 ++piece;
-                more = walk.next();
-                if (more) table = walk.table();
+                __syncwarp();                                // lane 0 has written this piece down
+                more = next(piece);
+                if (more) table = a.block_table + (size_t)at.table * a.table_stride;
             }
             if (more) ask();
         }
@@ -216,14 +246,18 @@ attn_shared_tc_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_con
         if (lane == 0) {
             const uint32_t idesc_s = umma_idesc_bf16(BQ, KT, false);      // S[128 x 64]  = Q (K-major) * K^T (K-major)
             const uint32_t idesc_o = umma_idesc_bf16(BQ, D, true);        // O[128 x D]  += P (tensor memory) * V (MN-major)
-            Walk<KT> ahead(a, plan);                         // the scores' way, up to a tile in front
-            bool more_s = ahead.next(), more_o = walk.next();
-            int m = 0, tile_s = 0, piece_s = 0;              // the next scores: tile, tile of their piece, piece
+            int m = 0, tile_s = 0, piece_s = 0;              // the next scores (up to a tile in front): tile, tile of their piece, piece
             int n = 0, tile_o = 0, piece_o = 0;              // the next weighted sum
+            bool more_s = piece_at(0, at), more_o = more_s;
+            int tiles_s = at.tiles, tiles_o = at.tiles;
             for (uint32_t spins = 0; more_o; ++spins) {
                 if (spins == SPIN_LIMIT << 4) { atomicExch(error_word, 63); break; }
+                if (more_s && tiles_s == 0 && mbar_test(found + 8 * (piece_s % PIECES), (piece_s / PIECES) & 1)) {
+                    tiles_s = pieces[piece_s % PIECES].tiles;
+                    more_s = tiles_s > 0;
+                }
                 // scores go to the buffer whose weights the sum before last used
-                if (more_s && m <= n + 1 && mbar_test(k_full + 8 * (m & 1), (m >> 1) & 1) && (tile_s || mbar_test(q_full + 8 * (piece_s & 1), (piece_s >> 1) & 1))) {
+                if (more_s && tiles_s && m <= n + 1 && mbar_test(k_full + 8 * (m & 1), (m >> 1) & 1) && (tile_s || mbar_test(q_full + 8 * (piece_s & 1), (piece_s >> 1) & 1))) {
                     const int s = m & 1;
                     tc_fence_after();
 #pragma unroll
@@ -234,11 +268,10 @@ attn_shared_tc_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_con
                     umma_commit(k_empty + 8 * s);              // the keys of this stage are free once these finish
                     umma_commit(s_full + 8 * s);
                     ++m;
-                    if (++tile_s == ahead.tiles) {
+                    if (++tile_s == tiles_s) {
                         umma_commit(q_done + 8 * (piece_s & 1));
-                        tile_s = 0;
+                        tile_s = tiles_s = 0;                  // the next piece's number of tiles is asked for when it is found
                         ++piece_s;
-                        more_s = ahead.next();
                     }
                     spins = 0;
                 }
@@ -251,10 +284,11 @@ attn_shared_tc_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_con
                     umma_commit(v_empty + 8 * s);
                     umma_commit(pv_done);
                     ++n;
-                    if (++tile_o == walk.tiles) {
+                    if (++tile_o == tiles_o) {
                         tile_o = 0;
                         ++piece_o;
-                        more_o = walk.next();
+                        more_o = piece_at(piece_o, at);
+                        tiles_o = at.tiles;
                     }
                     spins = 0;
                 }
@@ -266,16 +300,16 @@ attn_shared_tc_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_con
         const uint32_t lane_addr = tmem + ((uint32_t)(lg * 32) << 16);
         bool ok = true;
         int n = 0;
-        for (int piece = 0; ok && walk.next(); ++piece) {
-            const int rows = walk.rows * Hg, tiles = walk.tiles, lo = walk.lo, hi = walk.hi;
+        for (int piece = 0; ok && piece_at(piece, at); ++piece) {
+            const int rows = at.rows * Hg, tiles = at.tiles, lo = at.lo, hi = at.hi;
             const int copies = copies_of(1, rows), warps = 4 / copies, copy = lg / warps, col = copy * (KT / copies);
             const int mine = lg % warps * 32 + lane - (rows <= 16 && piece & 1 ? 16 : 0);      // the row
             const bool there = mine >= 0 && mine < rows, active = __any_sync(0xffffffffu, there);
             // a prefix's rows see no further than their own length; lanes beyond the rows hold anything
-            const int mine_hi = there ? min(hi, plan.keys[walk.row0 + mine / Hg]) : hi;
+            const int mine_hi = there ? min(hi, plan.keys[at.row0 + mine / Hg]) : hi;
             Row row{-INFINITY, 0.f};
             for (int i = 0; i < tiles && ok; ++i, ++n) {
-                const int s = n & 1, key = walk.key0 + i * KT;
+                const int s = n & 1, key = at.key0 + i * KT;
                 const uint32_t s_addr = lane_addr + S_COL + 64 * s;
                 if (!mbar_wait(s_full + 8 * s, (n >> 1) & 1)) { atomicExch(error_word, 68); ok = false; break; }
                 tc_fence_after();
@@ -291,9 +325,10 @@ attn_shared_tc_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_con
                     // Values in front of the piece's first or behind its last key may be anything (a page's unused part), and 0 * inf is no 0
                     if (!mbar_wait(v_full + 8 * s, (n >> 1) & 1)) { atomicExch(error_word, 62); ok = false; break; }
                     unsigned char* v = base + Q_BYTES + 2 * KV_BYTES + s * KV_BYTES;
-                    for (int id = tid; id < KT * HALVES * 8; id += 128) {
-                        const int chunk = id % 8, hb = id / 8 % HALVES, vr = id / (8 * HALVES);
-                        if (key + vr < lo || key + vr >= hi) *reinterpret_cast<uint4*>(v + hb * (KT * 128) + vr * 128 + chunk * 16) = make_uint4(0, 0, 0, 0);
+                    const int box = min(a.ps, KT), first = max(0, lo - key), last = min(KT, hi - key), end = min(KT, (last + box - 1) / box * box);
+                    for (int id = tid; id < (first + end - last) * HALVES * 8; id += 128) {
+                        const int row = id / (8 * HALVES), vr = row < first ? row : row - first + last, chunk = id % (8 * HALVES);
+                        *reinterpret_cast<uint4*>(v + chunk / 8 * (KT * 128) + vr * 128 + chunk % 8 * 16) = make_uint4(0, 0, 0, 0);
                     }
                     asm volatile("fence.proxy.async.shared::cta;\n" ::: "memory");
                 }
@@ -319,8 +354,8 @@ attn_shared_tc_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_con
             if (!mbar_wait(pv_done, (n - 1) & 1)) { atomicExch(error_word, 70); break; }
             tc_fence_after();
             if (active) {
-                const int rows_of = walk.prefix ? a.slot_rows : a.tail_rows, at = copy * rows + mine;
-                float4* to = reinterpret_cast<float4*>(walk.prefix ? a.o_prefix : a.o_tail) + (size_t)walk.place() * (D / 4) * rows_of + at;
+                const int rows_of = at.prefix ? a.slot_rows : a.tail_rows, line = copy * rows + mine;
+                float4* to = reinterpret_cast<float4*>(at.prefix ? a.o_prefix : a.o_tail) + (size_t)at.place * (D / 4) * rows_of + line;
 #pragma unroll 1
                 for (int c = 0; c < D / 32; ++c) {
                     uint32_t o[32];
@@ -332,7 +367,7 @@ attn_shared_tc_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_con
                             to[(size_t)(c * 8 + v4) * rows_of] = make_float4(__uint_as_float(o[4 * v4]), __uint_as_float(o[4 * v4 + 1]), __uint_as_float(o[4 * v4 + 2]), __uint_as_float(o[4 * v4 + 3]));
                     }
                 }
-                if (there) (walk.prefix ? a.ml_prefix : a.ml_tail)[(size_t)walk.place() * rows_of + at] = make_float2(row.m, row.l);
+                if (there) (at.prefix ? a.ml_prefix : a.ml_tail)[(size_t)at.place * rows_of + line] = make_float2(row.m, row.l);
             }
             tc_fence_before();
             mbar_arrive(o_free);
@@ -359,7 +394,7 @@ bool cache_map(const void* cache, long long rows, int D, int box, CUtensorMap* o
     return true;
 }
 
-// The queries [tokens, heads, D], rows of tokens `stride` elements apart, in boxes of a key head's query heads x 64
+// The queries [tokens, heads, D], tokens `stride` elements apart (whole heads), in boxes of a key head's query heads x 64 columns
 bool query_map(const void* q, int tokens, int H, int D, long long stride, int heads, CUtensorMap* out) {
     auto fn = sm100_host::encoder();
     if (!fn) return false;
@@ -396,7 +431,7 @@ MI_EXPORT int mi_attn_shared_tc(const void* q, int q_stride, int tokens, const v
                                 const int* shared_start, const int* shared_len, int G, int most, int H, int KV, int D, int ps, float scale, void* work,
                                 int* error_word, cudaStream_t stream) {
     if (R == 0) return 0;
-    if (!fits(R, G, H, KV, D, ps) || entries < 1 || tokens < 1 || q_stride % 8 || cache_rows > 0x7fffffff || (((uintptr_t)q | (uintptr_t)k_cache | (uintptr_t)v_cache | (uintptr_t)work) % 16)) return -2;
+    if (!fits(R, G, H, KV, D, ps) || entries < 1 || tokens < 1 || q_stride % D || cache_rows > 0x7fffffff || (((uintptr_t)q | (uintptr_t)k_cache | (uintptr_t)v_cache | (uintptr_t)work) % 16)) return -2;
     CUtensorMap qmap, kmap, vmap;
     if (!query_map(q, tokens, H, D, q_stride, H / KV, &qmap)) return -5;
     if (!cache_map(k_cache, cache_rows, D, ps < KT ? ps : KT, &kmap) || !cache_map(v_cache, cache_rows, D, ps < KT ? ps : KT, &vmap)) return -5;
@@ -404,7 +439,7 @@ MI_EXPORT int mi_attn_shared_tc(const void* q, int q_stride, int tokens, const v
     Args a{decode_segs, seg_q_start, seg_kv_len, block_table, table_rows, shared_start, shared_len, R, G, entries, most > 1 ? most : 1, table_stride, H, KV, ps,
            row_tiles_of(H, KV, most), tile_rows_of(H, KV), 1, slot_rows_of(H, KV, most), tail_rows_of(H, KV)};
     place_scratch(a, scratch(R, G, KV, D, a.row_tiles, a.slot_rows, a.tail_rows, blocks), work);
-    const auto bytes = [&](int ints) { return (size_t)BQ * D * 2 + 4 * (size_t)KT * D * 2 + 18 * 8 + (size_t)ints * 4 + 1024; };
+    const auto bytes = [&](int ints) { return (size_t)BQ * D * 2 + 4 * (size_t)KT * D * 2 + 26 * 8 + PIECES * sizeof(Piece) + (size_t)ints * 4 + 1024; };
     const size_t smem = bytes(plan_ints(G, R)), most_smem = bytes(6 * MAX_ENTITIES + 1);
     const float scale_log2 = scale * LOG2E;
 #define LAUNCH(DD) do { \

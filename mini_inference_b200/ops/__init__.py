@@ -666,8 +666,8 @@ class CudaOps:
         decode_segs[shared_start[g + 1] - 1] are group g (rows in no group stand alone), shared_len int32 [G]: the first so many keys of its rows are the
         same, and are read by the pages of the first row that has them all; max_shared_rows, on the host: rows of the largest group (rows beyond it are computed alone).  An entry
         without keys gets zeros.  The output [T, H D] has the entries' rows; others are left as they come.
-        Heads of 64 or 128 run on kernels that share; other heads, more than 4,096 entries and groups, and bfloat16 pages that neither divide 64 keys
-        nor are divided by them are computed row by row, by the rows' own pages."""
+        Heads of 64 or 128 run on kernels that share; other heads, more than 4,096 entries and groups, bfloat16 pages that neither divide 64 keys nor are divided
+        by them, and bfloat16 rows that do not lie whole heads apart are computed row by row, by the rows' own pages."""
         rows = getattr(meta, "table_rows", None)
         lists = (meta.decode_segs, meta.seg_q_start, meta.seg_kv_len, meta.shared_start, meta.shared_len)
         tables = (meta.block_table,) if rows is None else (meta.block_table, rows)
@@ -721,7 +721,7 @@ class CudaOps:
 
     def _shared_bytes(self, q, k_cache, v_cache, meta, H, KV, D):
         """Bytes of scratch of the kernel that reads shared prefixes once; not above 0: these rows are computed one by one."""
-        if not self.fast_attention or q.stride(0) % (16 // q.element_size()) or (q.data_ptr() | k_cache.data_ptr() | v_cache.data_ptr()) % 16:
+        if not self.fast_attention or q.stride(0) % (D if q.dtype is torch.bfloat16 else 4) or (q.data_ptr() | k_cache.data_ptr() | v_cache.data_ptr()) % 16:
             return 0
         size = self.lib.mi_attn_shared_tc_bytes if q.dtype is torch.bfloat16 else self.lib.mi_attn_shared_f32_bytes
         return size(meta.decode_segs.shape[0], meta.shared_len.shape[0], meta.max_shared_rows, H, KV, D, meta.page_size)
