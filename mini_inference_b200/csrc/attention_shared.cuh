@@ -177,14 +177,14 @@ struct Walk {
 struct __align__(16) Piece { int prefix, who, kvh, row0, rows, tiles, lo, hi, key0, place, table, spare; };
 
 // out[token of row r, heads of key head] from the row's pieces: a block per (row, key head), as many heads at a time as fill 128 threads with four columns each
-// (neighbouring heads in neighbouring threads).  A warp per head makes the weights of all pieces, then MERGE_PARTS groups of 128 threads take every
-// MERGE_PARTS-th piece, their rows read without waiting for one another, and are added up in the groups' order.
-constexpr int MERGE_PARTS = 2, MERGE_PIECES = 512;   // pieces whose weights are made at a time
-template <typename T, int D>
-__global__ void __launch_bounds__(128 * MERGE_PARTS) merge_kernel(const __grid_constant__ Args a, T* __restrict__ out) {
+// (neighbouring heads in neighbouring threads).  A warp per head makes the weights of all pieces, then PARTS groups of 128 threads take every
+// PARTS-th piece, their rows read without waiting for one another, and are added up in the groups' order.
+constexpr int MERGE_PIECES = 512;                      // pieces whose weights are made at a time
+template <typename T, int D, int PARTS>
+__global__ void __launch_bounds__(128 * PARTS, PARTS == 2 ? 4 : 1) merge_kernel(const __grid_constant__ Args a, T* __restrict__ out) {
     constexpr int HEADS = 512 / D;
     __shared__ float weight[MERGE_PIECES * HEADS], keep[HEADS], total[HEADS];
-    __shared__ float4 parts[MERGE_PARTS - 1][128];
+    __shared__ float4 parts[PARTS - 1][128];
     pdl_trigger();
     pdl_wait(out);
     const int r = blockIdx.x, kvh = blockIdx.y, Hg = a.H / a.KV, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
@@ -217,11 +217,11 @@ __global__ void __launch_bounds__(128 * MERGE_PARTS) merge_kernel(const __grid_c
             i -= n_p;
             return reinterpret_cast<const float4*>(a.o_tail) + ((at_t + (i >> shift_t)) * (D / 4) + c) * a.tail_rows + (i & (copies_t - 1)) * Hg + row_t + h;
         };
-        constexpr int EARLY = 8;                     // pieces of a thread that are asked for before their weights are there
+        constexpr int EARLY = 5;                     // pieces of a thread that are asked for before their weights are there
         float4 early[EARLY];
 #pragma unroll
         for (int k = 0; k < EARLY; ++k)
-            if (mine && part + k * MERGE_PARTS < n) early[k] = *rows_of(part + k * MERGE_PARTS);
+            if (mine && part + k * PARTS < n) early[k] = *rows_of(part + k * PARTS);
         for (int i0 = 0; i0 < max(n, 1); i0 += MERGE_PIECES) {
             const int now = min(MERGE_PIECES, n - i0);
             if (warp < heads) {
@@ -260,11 +260,11 @@ __global__ void __launch_bounds__(128 * MERGE_PARTS) merge_kernel(const __grid_c
                 if (i0 == 0) {
 #pragma unroll
                     for (int k = 0; k < EARLY; ++k)
-                        if (part + k * MERGE_PARTS < now) add(early[k], weight[(part + k * MERGE_PARTS) * HEADS + h]);
-                    i += EARLY * MERGE_PARTS;
+                        if (part + k * PARTS < now) add(early[k], weight[(part + k * PARTS) * HEADS + h]);
+                    i += EARLY * PARTS;
                 }
 #pragma unroll 4
-                for (; i < end; i += MERGE_PARTS) add(*rows_of(i), weight[(i - i0) * HEADS + h]);
+                for (; i < end; i += PARTS) add(*rows_of(i), weight[(i - i0) * HEADS + h]);
             }
             __syncthreads();
         }
@@ -272,7 +272,7 @@ __global__ void __launch_bounds__(128 * MERGE_PARTS) merge_kernel(const __grid_c
         __syncthreads();
         if (part == 0 && mine) {
 #pragma unroll
-            for (int k = 0; k < MERGE_PARTS - 1; ++k) { const float4 v = parts[k][id]; o.x += v.x; o.y += v.y; o.z += v.z; o.w += v.w; }
+            for (int k = 0; k < PARTS - 1; ++k) { const float4 v = parts[k][id]; o.x += v.x; o.y += v.y; o.z += v.z; o.w += v.w; }
             const float sum = total[h], inv = sum > 0.f ? 1.f / sum : sum == 0.f ? 0.f : sum;      // no key at all: 0; NaN stays
             T* to = out + ((size_t)rec.token * a.H + (size_t)kvh * Hg + h0 + h) * D + 4 * c;
             store2(to, o.x * inv, o.y * inv);
@@ -280,6 +280,11 @@ __global__ void __launch_bounds__(128 * MERGE_PARTS) merge_kernel(const __grid_c
         }
         __syncthreads();
     }
+}
+// Few rows leave SMs empty, and there eight groups of threads a row are the faster ones; many rows want more blocks an SM.
+template <typename T, int D> inline cudaError_t merge(const Args& a, T* out, cudaStream_t stream) {
+    if ((long long)a.R * a.KV <= device_sms()) return launch_pdl(merge_kernel<T, D, 8>, dim3(a.R, a.KV), dim3(1024), 0, stream, a, out);
+    return launch_pdl(merge_kernel<T, D, 2>, dim3(a.R, a.KV), dim3(256), 0, stream, a, out);
 }
 
 // Lets a kernel have `bytes` of shared memory, once a device (asking again costs a call about 2 us)

@@ -193,7 +193,7 @@ MI_EXPORT int mi_attn_shared_f32(const float* q, int q_stride, const float* k_ca
         cudaError_t e = allow_shared(attn_shared_f32_kernel<DD>, (int)(smem + (6 * MAX_ENTITIES + 1) * 4), done); \
         if (e == cudaSuccess) e = launch_pdl(attn_shared_f32_kernel<DD>, dim3(blocks), dim3(THREADS), smem + plan, stream, a, q, (long long)q_stride, k_cache, v_cache, \
                                              scale_log2); \
-        if (e == cudaSuccess) e = launch_pdl(merge_kernel<float, DD>, dim3(R, KV), dim3(128 * MERGE_PARTS), 0, stream, a, out); \
+        if (e == cudaSuccess) e = merge<float, DD>(a, out, stream); \
         return (int)e; \
     } while (0)
     if (D == 128) LAUNCH(128);

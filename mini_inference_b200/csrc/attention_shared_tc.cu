@@ -446,7 +446,7 @@ MI_EXPORT int mi_attn_shared_tc(const void* q, int q_stride, int tokens, const v
         static unsigned long long done = 0; \
         cudaError_t e = allow_shared(attn_shared_tc_kernel<DD>, (int)most_smem, done); \
         if (e == cudaSuccess) e = launch_pdl(attn_shared_tc_kernel<DD>, dim3(blocks), dim3(THREADS), smem, stream, qmap, kmap, vmap, a, scale_log2, error_word); \
-        if (e == cudaSuccess) e = launch_pdl(merge_kernel<__nv_bfloat16, DD>, dim3(R, KV), dim3(128 * MERGE_PARTS), 0, stream, a, (__nv_bfloat16*)out); \
+        if (e == cudaSuccess) e = merge<__nv_bfloat16, DD>(a, (__nv_bfloat16*)out, stream); \
         return (int)e; \
     } while (0)
     if (D == 128) LAUNCH(128);
