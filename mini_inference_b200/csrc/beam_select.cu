@@ -9,23 +9,45 @@
 // would swap two neighbours that lie 0.05 apart once in some hundred thousand pairs, a step of 64 beams has a thousand.  Within a row the logits
 // themselves decide, exactly.
 //
-// Two launches.  beam_slice_kernel: a block takes a slice of one row into registers once, and leaves the slice's maximum, its sum of exponentials and
-// its `num` largest logits in order.  The num / 8-th largest of each warp's 32 threads' maxima, the least of the eight, is a bound that at least num
-// logits reach; what reaches it (a few more than num) goes to shared memory and every entry counts those before it.  Where more reach it than fit (many
-// equal logits) the num-th of those that found room is the next bound: all candidates differ in their order, so each turn has at least CAP - num fewer.  beam_merge_kernel: a block per group joins the slices' sums, and chooses among their sorted lists the
-// same way: a bound from the lists' heads, then a thread per list follows its list down to the bound.
+// Two launches.  beam_slice_kernel: a block streams a slice of one row once (asynchronous copies, up to three tiles in front) and keeps its sum of exponentials and, per
+// thread, the largest logit.  The num / 8-th largest of each warp's 32 threads, the least of the eight, is a bound that num threads reach; the num-th of those that do is a
+// better one, and only the logits of threads whose largest reaches that are read again (from the L2 cache, 1 / 16 of the slice for num = 16) and put in order by counting.
+// Keeping candidates while streaming cost three instructions a logit and ten for each that a bound from the first tiles lets through: 24 us instead of 19 at 64 x 151,936.
+// Where more reach the bound than fit (many equal logits) the num-th of those that found room is the next bound: all candidates differ in their order, so
+// each turn has at least CAP - num fewer.
+// beam_merge_kernel: a block per group joins the slices' sums, finds a bound from the first, second, fourth, ... candidates of their sorted lists, and follows each list down to it.
+// Bounds from the first ones alone let every list of a beam far ahead of the others through: 16 us instead of 8 for 16 beams with scores some units apart.
+// Time at 64 rows x 151,936, num 16: 24 us (38.9 MB: 6 us); 38 instructions a logit, 18 of them the exponential, keep two of three issue slots busy.
+// 4 x 32,768: 8 us, two launches with everything cold.
 #include "common.cuh"
+#include <algorithm>
+#include <float.h>
 #include <math.h>
 
 using namespace mi;
 
 namespace {
 
-constexpr int NT = 256, CAP = 1024, BASES = 128;                 // threads of a block (at least MAX_NUM); candidates that fit in shared memory
+constexpr int NT = 256, EPT = 8, TILE = NT * EPT;                // threads of a block (at least MAX_NUM), logits of a thread and of all at a time
+constexpr int AHEAD = 4, BLOCKS = 4;                              // tiles in shared memory; blocks an SM
+constexpr int CAP = 1024, BASES = 128;                           // candidates that fit in shared memory; rows of a group whose base does
 constexpr int MAX_NUM = 128, WARPS = NT / 32;
 typedef unsigned long long u64;
 
-struct __align__(16) SliceSum { double sum; float top; int count; };
+__device__ __forceinline__ float max_or_nan(float a, float b, float c) { float d; asm("max.NaN.f32 %0, %1, %2, %3;\n" : "=f"(d) : "f"(a), "f"(b), "f"(c)); return d; }
+// A sum of exponentials in units of 2^at (at a whole number: units are changed without rounding) or, where logits are large, e^at.
+// at NaN: the row offers nothing; -inf: no logit above -inf
+struct __align__(16) SliceSum { double sum; float at; int binary; };
+__device__ __forceinline__ double log_unit(const SliceSum& s) { return s.binary ? (double)s.at * 0.6931471805599453 : (double)s.at; }
+__device__ __forceinline__ double in_units(const SliceSum& s, const SliceSum& of) {      // of is the larger unit
+    if (s.at == -INFINITY) return 0.;
+    if (s.binary && of.binary) return s.sum * __hiloint2double((1023 + max((int)(s.at - of.at), -1000)) << 20, 0);
+    return s.sum * exp(log_unit(s) - log_unit(of));
+}
+__device__ __forceinline__ SliceSum larger_unit(const SliceSum& a, const SliceSum& b) {  // sum aside; NaN is the largest
+    if (a.binary && b.binary) return SliceSum{0., max_or_nan(a.at, b.at, -INFINITY), 1};
+    return isnan(a.at) || isnan(b.at) ? SliceSum{0., NAN, 1} : log_unit(a) >= log_unit(b) ? a : b;
+}
 
 // larger logit first, then the lower token; 0 is below every candidate's key
 __device__ __forceinline__ u64 logit_key(float v, int token) {
@@ -39,26 +61,37 @@ __device__ __forceinline__ float key_logit(u64 key) {
 }
 __device__ __forceinline__ int key_token(u64 key) { return (int)(0xffffffffu - (uint32_t)key); }
 
-template <typename T> __device__ __forceinline__ T warp_largest(T v) {
+__device__ __forceinline__ float warp_largest(float v) { float d; asm("redux.sync.max.f32 %0, %1, 0xffffffff;\n" : "=f"(d) : "f"(v)); return d; }
+__device__ __forceinline__ float warp_least(float v) { float d; asm("redux.sync.min.f32 %0, %1, 0xffffffff;\n" : "=f"(d) : "f"(v)); return d; }
+__device__ __forceinline__ double warp_largest(double v) {
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) { const T w = __shfl_xor_sync(0xffffffffu, v, o); v = w > v ? w : v; }
+    for (int o = 16; o > 0; o >>= 1) { const double w = __shfl_xor_sync(0xffffffffu, v, o); v = w > v ? w : v; }
     return v;
 }
-// The `turn`-th largest of a warp's values (lowest: below all of them), and the largest
-template <typename T> __device__ __forceinline__ T warp_nth(T mine, int turn, T lowest, T& largest) {
-    T best = largest = warp_largest(mine);
-    for (int k = 1; k < turn; ++k) {                 // once more without the lane that had it
-        const uint32_t who = __ballot_sync(0xffffffffu, mine == best);
-        if ((threadIdx.x & 31) == __ffs(who) - 1) mine = lowest;
-        best = warp_largest(mine);
+// The n-th largest of a warp's values
+__device__ __forceinline__ float warp_nth(float mine, int n) {
+    if (n == 1) return warp_largest(mine);
+    const int lane = threadIdx.x & 31;
+    int before = 0;
+#pragma unroll 8
+    for (int o = 1; o < 32; ++o) {
+        const float other = __shfl_xor_sync(0xffffffffu, mine, o);
+        before += (other > mine) | ((other == mine) & ((lane ^ o) < lane));
     }
-    return best;
+    return __shfl_sync(0xffffffffu, mine, __ffs(__ballot_sync(0xffffffffu, before == n - 1)) - 1);
+}
+__device__ __forceinline__ double warp_nth(double mine, int n) {
+    for (int k = 1;; ++k) {
+        const double best = warp_largest(mine);
+        if (k == n) return best;
+        const uint32_t who = __ballot_sync(0xffffffffu, mine == best);      // once more without the lane that had it
+        if ((threadIdx.x & 31) == __ffs(who) - 1) mine = -(double)INFINITY;
+    }
 }
 // A bound that at least num (<= NT) of the threads' values reach: the least over the warps of their num / 8-th largest
 __device__ __forceinline__ int turns(int num) { return (num + WARPS - 1) / WARPS; }
 __device__ __forceinline__ double threshold(double mine, int num, double* scratch) {
-    double largest;
-    double best = warp_nth(mine, turns(num), -(double)INFINITY, largest);
+    double best = warp_nth(mine, turns(num));
     __syncthreads();
     if ((threadIdx.x & 31) == 0) scratch[threadIdx.x >> 5] = best;
     __syncthreads();
@@ -67,12 +100,12 @@ __device__ __forceinline__ double threshold(double mine, int num, double* scratc
     return best;
 }
 
-// e^(x - m) for logits x <= m, |m| <= 1024, with errors of about 5e-10 of it, as a leading and a small part: 2^t, t = n + j / 32 + r, is 2^n times a table's 2^(j / 32)
-// times a polynomial in r, |r| <= 1/64 (table-driven, after Tang).  m log2(e) is split into a multiple of 2^-12, to which j / 32 is added without
-// rounding, and the rest, so that r is off by 2^-31 or so.  The table is spread over a warp's lanes.
+// e^x for logits |x| <= 1024 up to a largest one, in units of 2^at, with errors of about 5e-10 of it, as a leading and a small part: 2^t, t = x log2(e) - at = n + j / 32 + r,
+// is 2^n times a table's 2^(j / 32) times a polynomial in r, |r| <= 1/64 (table-driven, after Tang).  at is a whole number, so that taking it and
+// n + j / 32 away leaves nothing to round but r itself, 2^-31 or so.  The table is spread over a warp's lanes.
 constexpr float LOG2E_HI = 0x1.715476p+0f, LOG2E_LO = 0x1.4ae0cp-26f;
-__device__ const float2 POWERS[32] = {        // 2^(j / 32) and what its rounding left
-    {1.f, 0.f}, {1.0218971967697144f, -4.81155986e-08f}, {1.0442737340927124f, 4.83347016e-08f}, {1.0671404600143433f, -5.93375198e-08f},
+__device__ const float2 POWERS[32] = {        // 2^(j / 32) and what its rounding left (not 0, 2^-40: its exponent is added to)
+    {1.f, 1e-12f}, {1.0218971967697144f, -4.81155986e-08f}, {1.0442737340927124f, 4.83347016e-08f}, {1.0671404600143433f, -5.93375198e-08f},
     {1.0905077457427979f, -1.30775399e-08f}, {1.114386796951294f, -5.43554002e-08f}, {1.1387885808944702f, 5.38622231e-08f}, {1.1637248992919922f, -4.05144149e-08f},
     {1.1892070770263672f, 3.79763527e-08f}, {1.215247392654419f, -3.26739489e-08f}, {1.2418577671051025f, 4.4968381e-08f}, {1.2690509557724f, 1.41933332e-09f},
     {1.2968395948410034f, -4.01899953e-08f}, {1.3252366781234741f, -3.49637332e-08f}, {1.3542555570602417f, -1.01233493e-08f}, {1.3839099407196045f, -5.87557736e-08f},
@@ -82,139 +115,225 @@ __device__ const float2 POWERS[32] = {        // 2^(j / 32) and what its roundin
     {1.8340080976486206f, -1.1239278e-08f}, {1.8741676807403564f, -4.66300563e-08f}, {1.9152065515518188f, 9.84532811e-09f}, {1.9571441411972046f, -1.70218044e-08f}};
 struct Exponential {
     float2 power;                                    // of this lane
-    float m_hi, m_lo, m_32, least;
+    float at, least;
     __device__ __forceinline__ Exponential(float m, const float2& power_) : power(power_) {
-        const double y = (double)m * 1.4426950408889634074;
-        m_hi = (float)(rint(y * 4096.) * (1. / 4096.));
-        m_lo = (float)(y - (double)m_hi);
-        m_32 = -32.f * m_hi;
+        at = rintf(m * LOG2E_HI);
         least = m - 44.f;                            // e^-44 = 2^-63: logits below it (-inf among them) count as that
     }
     // of two logits at once: adds their leading parts to sum and the rest to rest
     __device__ __forceinline__ void operator()(float x0, float x1, double& sum, float& rest) const {
-        const float2 x = make_float2(fmaxf(x0, least), fmaxf(x1, least)), magic = make_float2(12582912.f, 12582912.f);
-        const float2 z = __fadd2_rn(__ffma2_rn(x, make_float2(32.f * LOG2E_HI, 32.f * LOG2E_HI), make_float2(m_32, m_32)), magic);      // its last bits: 32 t rounded to a whole number
-        const float2 k = __fadd2_rn(z, make_float2(-12582912.f, -12582912.f));
-        const float2 c = __ffma2_rn(k, make_float2(-1.f / 32.f, -1.f / 32.f), make_float2(-m_hi, -m_hi));
-        const float2 r = __fadd2_rn(__ffma2_rn(x, make_float2(LOG2E_LO, LOG2E_LO), __ffma2_rn(x, make_float2(LOG2E_HI, LOG2E_HI), c)), make_float2(-m_lo, -m_lo));
-        float2 p = __ffma2_rn(r, make_float2(0x1.3b2ab6p-7f, 0x1.3b2ab6p-7f), make_float2(0x1.c6b08ep-5f, 0x1.c6b08ep-5f));                // ln(2)^i / i!
-        p = __ffma2_rn(r, p, make_float2(0x1.ebfbep-3f, 0x1.ebfbep-3f));
+        constexpr float MAGIC = 12582912.f;          // its last bit is 1, so adding it rounds to a whole number
+        const float start = fmaf(-32.f, at, MAGIC), back = MAGIC / 32.f - at;      // both exact
+        const float2 x = make_float2(fmaxf(x0, least), fmaxf(x1, least));
+        const float2 z = __ffma2_rn(x, make_float2(32.f * LOG2E_HI, 32.f * LOG2E_HI), make_float2(start, start));      // its last bits: 32 t rounded to a whole number
+        const float2 c = __ffma2_rn(z, make_float2(-1.f / 32.f, -1.f / 32.f), make_float2(back, back));                 // -(at + that / 32), exact
+        const float2 r = __ffma2_rn(x, make_float2(LOG2E_LO, LOG2E_LO), __ffma2_rn(x, make_float2(LOG2E_HI, LOG2E_HI), c));
+        float2 p = __ffma2_rn(r, make_float2(0x1.c6b08ep-5f, 0x1.c6b08ep-5f), make_float2(SQUARE, SQUARE));             // ln(2)^i / i!
         p = __fmul2_rn(r, __ffma2_rn(r, p, make_float2(0x1.62e43p-1f, 0x1.62e43p-1f)));
         const int k0 = __float_as_int(z.x), k1 = __float_as_int(z.y);      // the magic number's own last bits are 0
-        const float2 hi = make_float2(__shfl_sync(0xffffffffu, power.x, k0), __shfl_sync(0xffffffffu, power.x, k1));
-        const float2 lo = make_float2(__shfl_sync(0xffffffffu, power.y, k0), __shfl_sync(0xffffffffu, power.y, k1));
-        // 2^floor(k / 32): bits 5 and up of k (mod 2^8) into the exponent
-        const float2 scale = make_float2(__int_as_float(((k0 >> 5) + 127) << 23), __int_as_float(((k1 >> 5) + 127) << 23));
-        const float2 lead = __fmul2_rn(hi, scale), small = __fmul2_rn(__ffma2_rn(hi, p, lo), scale);
-        sum += (double)lead.x;
-        sum += (double)lead.y;
+        const auto times = [](float v, int k) { return __int_as_float(__float_as_int(v) + ((k & ~31) << 18)); };      // 2^floor(k / 32) v: bits 5 and up of k added to the exponent
+        const float2 hi = make_float2(times(__shfl_sync(0xffffffffu, power.x, k0), k0), times(__shfl_sync(0xffffffffu, power.x, k1), k1));
+        const float2 lo = make_float2(times(__shfl_sync(0xffffffffu, power.y, k0), k0), times(__shfl_sync(0xffffffffu, power.y, k1), k1));
+        const float2 small = __ffma2_rn(hi, p, lo);
+        sum += (double)hi.x;
+        sum += (double)hi.y;
         rest += small.x + small.y;
     }
+    // r^4 ln(2)^4 / 24 over |r| <= 1/64 is r^2 ln(2)^4 / (24 64^2) to 1.5e-10
+    static constexpr float SQUARE = (float)(0.24022650695910072 + 0.23083509858308343 / (24. * 4096.));
 };
 
-// EPT logits a thread, four neighbours at a time
-template <int EPT>
-__global__ void __launch_bounds__(NT, 4) beam_slice_kernel(const float* __restrict__ logits, long long ld, int vocab, int num, SliceSum* __restrict__ sums,
+
+__device__ __forceinline__ void cp_async16(float* to, const float* from) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;\n" :: "r"((uint32_t)__cvta_generic_to_shared(to)), "l"(from) : "memory");
+}
+__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;\n" ::: "memory"); }
+template <int N> __device__ __forceinline__ void cp_async_wait() { asm volatile("cp.async.wait_group %0;\n" :: "n"(N) : "memory"); }
+
+// The best num of the first n (<= CAP) of found, to its front and in order.  Returns how many.
+__device__ __forceinline__ int keep_best(u64* found, int n, int num) {
+    constexpr int MINE = CAP / NT;
+    u64 mine[MINE];
+    int before[MINE];
+#pragma unroll
+    for (int e = 0; e < MINE; ++e) {
+        const int i = threadIdx.x + e * NT;
+        before[e] = num;
+        if (i < n) {
+            mine[e] = found[i];
+            before[e] = 0;
+#pragma unroll 8
+            for (int o = 0; o < n; ++o) before[e] += found[o] > mine[e];
+        }
+    }
+    __syncthreads();
+#pragma unroll
+    for (int e = 0; e < MINE; ++e)
+        if (before[e] < num) found[before[e]] = mine[e];
+    __syncthreads();
+    return min(n, num);
+}
+
+// A block takes `per` logits of a row, TILE at a time; AHEAD tiles are on their way to shared memory meanwhile, each thread reading what it asked for itself.
+// Each warp has its own sum, in units of its own; nothing else is kept but each thread's largest.
+__global__ void __launch_bounds__(NT, BLOCKS) beam_slice_kernel(const float* __restrict__ logits, long long ld, int vocab, int per, int num, SliceSum* __restrict__ sums,
                                                            u64* __restrict__ keys) {
-    __shared__ float tops[WARPS], bounds[WARPS];
-    __shared__ double parts[WARPS];
-    __shared__ u64 found[CAP], floor_of;
-    __shared__ int count;
+    extern __shared__ __align__(16) float ring[];    // [AHEAD][EPT / 4][NT][4]; then candidates
+    __shared__ float bounds[WARPS];
+    __shared__ SliceSum parts[WARPS];
+    __shared__ int count, lists;
+    __shared__ float2 hits[NT];                      // a thread's largest logit, and the thread
+    __shared__ float better;
     pdl_trigger();
     const float2 power = POWERS[threadIdx.x & 31];
+    if (threadIdx.x == 0) count = lists = 0;
     pdl_wait(logits);
-    const int r = blockIdx.y, slice = blockIdx.x, slices = gridDim.x, base = slice * NT * EPT, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    const float* row = logits + (long long)r * ld;
-    const bool vec = ((uintptr_t)row & 15) == 0;
-    const auto index = [&](int e) { return base + ((e >> 2) * NT + (int)threadIdx.x) * 4 + (e & 3); };
-    float x[EPT];
+    const int r = blockIdx.y, slice = blockIdx.x, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    // the row from a 16-byte boundary on, up to three numbers in front of it
+    const int off = (int)((uintptr_t)(logits + (long long)r * ld) >> 2 & 3);
+    const float* row = logits + (long long)r * ld - off;
+    const int begin = max(off, slice * per), end = min((slice + 1) * per, vocab + off), tiles = max(1, (end - slice * per + TILE - 1) / TILE);
+    const auto fetch = [&](int tile) {
+        if (tile < tiles) {
+            float* to = ring + (tile % AHEAD * TILE + (int)threadIdx.x * 4);
+            const int i0 = slice * per + tile * TILE + (int)threadIdx.x * 4;
 #pragma unroll
-    for (int k = 0; k < EPT / 4; ++k) {
-        const int i = index(4 * k);
-        if (vec && i + 3 < vocab) {
-            load16(row + i, x + 4 * k);
-        } else {
+            for (int k = 0; k < EPT / 4; ++k) {
+                const int i = i0 + k * NT * 4;
+                if (i >= begin && i + 3 < end) {
+                    cp_async16(to + k * NT * 4, row + i);
+                } else {
 #pragma unroll
-            for (int e = 0; e < 4; ++e) x[4 * k + e] = i + e < vocab ? row[i + e] : -INFINITY;
-        }
-    }
-    float top = -INFINITY;
-    bool bad = false;
-#pragma unroll
-    for (int e = 0; e < EPT; ++e) {
-        bad |= !(x[e] < INFINITY);
-        top = fmaxf(top, x[e]);
-    }
-    if (bad) top = INFINITY;
-    float largest;
-    const float nth = warp_nth(top, turns(num), -INFINITY, largest);
-    if (threadIdx.x == 0) count = 0;
-    if (lane == 0) { tops[warp] = largest; bounds[warp] = nth; }
-    __syncthreads();
-    float m = tops[0], least = bounds[0];
-#pragma unroll
-    for (int w = 1; w < WARPS; ++w) { m = fmaxf(m, tops[w]); least = fminf(least, bounds[w]); }
-    SliceSum* out = sums + (size_t)r * slices + slice;
-    u64* best = keys + ((size_t)r * slices + slice) * num;
-    if (!(fabsf(m) < INFINITY)) {                    // NaN or +inf (the row offers nothing), or nothing above -inf
-        if (threadIdx.x == 0) *out = SliceSum{m == -INFINITY ? 0. : (double)NAN, m, 0};
-        for (int k = threadIdx.x; k < num; k += NT) best[k] = 0;
-        return;
-    }
-    double sum = 0.;
-    if (fabsf(m) <= 1024.f) {
-        const Exponential exponential(m, power);
-        float rest = 0.f;
-#pragma unroll
-        for (int e = 0; e < EPT; e += 2) exponential(x[e], x[e + 1], sum, rest);
-        sum += (double)rest;
-    } else {
-#pragma unroll
-        for (int e = 0; e < EPT; ++e) sum += exp((double)x[e] - (double)m);
-    }
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-    if (lane == 0) parts[warp] = sum;
-    uint32_t hits = 0;                               // few of a thread's logits reach the bound: those are read once more
-#pragma unroll
-    for (int e = 0; e < EPT; ++e) hits |= (x[e] >= least && x[e] > -INFINITY ? 1u : 0u) << e;
-    int n;
-    for (u64 floor_key = 0;;) {
-        for (uint32_t left = hits; left; left &= left - 1) {
-            const int i = index(__ffs(left) - 1);
-            const u64 key = logit_key(row[i] + 0.f, i);      // -0 is 0
-            if (key >= floor_key) {
-                const int at = atomicAdd(&count, 1);
-                if (at < CAP) found[at] = key;
+                    for (int e = 0; e < 4; ++e) to[k * NT * 4 + e] = i + e >= begin && i + e < end ? row[i + e] : -INFINITY;
+                }
             }
         }
-        __syncthreads();
-        n = count;
-        if (n <= CAP) break;
-        for (int i = threadIdx.x; i < CAP; i += NT) {
-            const u64 mine = found[i];
+        cp_async_commit();
+    };
+    for (int tile = 0; tile < AHEAD - 1; ++tile) fetch(tile);
+    Exponential exponential(0.f, power);
+    float near = -INFINITY, mine = -INFINITY;        // what the warp's units are for (the largest logit when they were taken); this thread's largest
+    SliceSum all{0., -INFINITY, 1};
+    for (int tile = 0; tile < tiles; ++tile) {
+        cp_async_wait<AHEAD - 2>();
+        float x[EPT];
+#pragma unroll
+        for (int k = 0; k < EPT / 4; ++k) load16(ring + (tile % AHEAD * TILE + (k * NT + (int)threadIdx.x) * 4), x + 4 * k);
+        fetch(tile + AHEAD - 1);
+        float top = x[0];
+#pragma unroll
+        for (int e = 1; e + 1 < EPT; e += 2) top = max_or_nan(top, x[e], x[e + 1]);
+        top = max_or_nan(top, x[EPT - 1], -INFINITY);
+        if (!(top < INFINITY)) top = INFINITY;       // NaN too: the row offers nothing
+        mine = fmaxf(mine, top);
+        if (__any_sync(0xffffffffu, top > near + 20.f)) {      // other units: not often
+            near = warp_largest(top);
+            if (near < INFINITY) {
+                SliceSum now{0., near, 0};
+                if (fabsf(near) <= 1000.f) {
+                    exponential = Exponential(near, power);
+                    now = SliceSum{0., exponential.at, 1};
+                }
+                now.sum = in_units(all, now);
+                all = now;
+            }
+        }
+        if (fabsf(near) <= 1000.f) {
+            float rest = 0.f;
+#pragma unroll
+            for (int e = 0; e < EPT; e += 2) exponential(x[e], x[e + 1], all.sum, rest);
+            all.sum += (double)rest;
+        } else if (fabsf(near) < INFINITY) {
+#pragma unroll 1
+            for (int k = 0; k < EPT; ++k) {
+                float v = x[0];
+#pragma unroll
+                for (int e = 1; e < EPT; ++e) v = k == e ? x[e] : v;
+                all.sum += exp((double)v - (double)near);
+            }
+        }
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) all.sum += __shfl_xor_sync(0xffffffffu, all.sum, o);
+    const float largest = warp_largest(mine), nth = warp_nth(mine, turns(num));
+    if (lane == 0) {
+        if (largest == INFINITY) all = SliceSum{0., NAN, 1};
+        parts[warp] = all;
+        bounds[warp] = nth;
+    }
+    __syncthreads();
+    SliceSum whole = parts[lane % WARPS];
+    const bool bad = __any_sync(0xffffffffu, isnan(whole.at)), none = !__any_sync(0xffffffffu, whole.at > -INFINITY);
+    SliceSum* out = sums + (size_t)r * gridDim.x + slice;
+    const size_t list = (size_t)r * gridDim.x + slice, all_lists = (size_t)gridDim.y * gridDim.x;      // a list's k-th candidate is keys[k all_lists + list]
+    if (bad || none) {
+        if (threadIdx.x == 0) *out = SliceSum{0., bad ? NAN : -INFINITY, 1};
+        for (int k = threadIdx.x; k < num; k += NT) keys[k * all_lists + list] = 0;
+        return;
+    }
+    // num threads' largest reach the bound.  The num-th of those that do is a better one; the logits of the threads that reach that are looked at once more.
+    float least = fmaxf(warp_least(bounds[lane % WARPS]), -FLT_MAX);
+    if (mine >= least) hits[atomicAdd(&lists, 1)] = make_float2(mine, __int_as_float((int)threadIdx.x));
+    __syncthreads();
+    const int reach = lists, quads = tiles * (EPT / 4);
+    if (reach >= num && reach * quads > NT) {        // (fewer than num: a row with few logits above -inf)
+        if ((int)threadIdx.x < reach) {
+            const float2 me = hits[threadIdx.x];
             int before = 0;
-            for (int o = 0; o < CAP; ++o) before += found[o] > mine;
-            if (before == num - 1) floor_of = mine;
+#pragma unroll 4
+            for (int o = 0; o < reach; ++o) { const float2 other = hits[o]; before += (other.x > me.x) | ((other.x == me.x) & (o < (int)threadIdx.x)); }
+            if (before == num - 1) better = me.x;
         }
         __syncthreads();
-        floor_key = floor_of;
+        least = better;
+    }
+    u64* found = reinterpret_cast<u64*>(ring);       // nothing is on its way any more
+    u64 floor_key = 0;
+    for (;;) {
+        for (int q = threadIdx.x; q < reach * quads; q += NT) {      // a quad a thread
+            const float2 hit = hits[q / quads];
+            if (hit.x < least) continue;
+            const int i = slice * per + (q % quads * NT + __float_as_int(hit.y)) * 4;
+            float x[4];
+            if (i >= begin && i + 3 < end) {
+                load16(row + i, x);
+            } else {
+#pragma unroll
+                for (int e = 0; e < 4; ++e) x[e] = i + e >= begin && i + e < end ? row[i + e] : -INFINITY;
+            }
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+                if (x[e] >= least) {
+                    const u64 key = logit_key(x[e] + 0.f, i + e - off);      // -0 is 0
+                    if (key < floor_key) continue;
+                    const int p = atomicAdd(&count, 1);
+                    if (p < CAP) found[p] = key;
+                }
+        }
+        __syncthreads();
+        const int n = keep_best(found, min(count, CAP), num);
+        if (count <= CAP) {
+            for (int k = threadIdx.x; k < num; k += NT) keys[k * all_lists + list] = k < n ? found[k] : 0;
+            break;
+        }
+        floor_key = found[num - 1];                  // many equal logits: once more, from the num-th of those that found room on
+        __syncthreads();
         if (threadIdx.x == 0) count = 0;
         __syncthreads();
     }
-    for (int i = threadIdx.x; i < n; i += NT) {
-        const u64 mine = found[i];
-        int before = 0;
-#pragma unroll 8
-        for (int o = 0; o < n; ++o) before += found[o] > mine;
-        if (before < num) best[before] = mine;
-    }
-    for (int k = n + threadIdx.x; k < num; k += NT) best[k] = 0;
-    if (threadIdx.x == 0) {
-        for (int w = 1; w < WARPS; ++w) sum += parts[w];
-        *out = SliceSum{sum, m, min(n, num)};
+    if (warp == 0) {
+        SliceSum unit = whole;
+#pragma unroll
+        for (int o = WARPS / 2; o > 0; o >>= 1)
+            unit = larger_unit(unit, SliceSum{0., __shfl_xor_sync(0xffffffffu, unit.at, o), __shfl_xor_sync(0xffffffffu, unit.binary, o)});
+        unit.sum = in_units(whole, unit);
+#pragma unroll
+        for (int o = WARPS / 2; o > 0; o >>= 1) unit.sum += __shfl_xor_sync(0xffffffffu, unit.sum, o);
+        if (lane == 0) *out = unit;
     }
 }
+
+static_assert(AHEAD * TILE * 4 >= CAP * (int)sizeof(u64) && AHEAD * TILE * 4 <= 40 * 1024, "");
 
 struct Candidate { double value; int row; u64 key; };
 __device__ __forceinline__ bool goes_before(const Candidate& a, const Candidate& b) {
@@ -238,6 +357,7 @@ __global__ void __launch_bounds__(NT) beam_merge_kernel(const SliceSum* sums, co
                                                         const int* __restrict__ group_start, double* base, float* __restrict__ values, int* __restrict__ out_rows,
                                                         int* __restrict__ out_tokens) {
     __shared__ double scratch[WARPS], near_base[BASES];
+    __shared__ float bounds[WARPS];
     __shared__ Found found;
     __shared__ Candidate bound;
     __shared__ int count;
@@ -245,58 +365,92 @@ __global__ void __launch_bounds__(NT) beam_merge_kernel(const SliceSum* sums, co
     pdl_wait(scores, group_start);
     const int g = blockIdx.x, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int a = max(0, min(group_start[g], rows)), b = max(a, min(group_start[g + 1], rows));
-    // s[r] - lse[r], a warp per row
-    for (int r = a + warp; r < b; r += WARPS) {
-        const SliceSum* mine = sums + (size_t)r * slices;
-        float m = -INFINITY;
-        for (int i = lane; i < slices; i += 32) m = fmaxf(m, mine[i].top);
-        m = warp_max(m);
-        double sum = 0.;
-        for (int i = lane; i < slices; i += 32) sum += mine[i].sum * (mine[i].top == -INFINITY ? 1. : exp((double)mine[i].top - (double)m));
+    // list i: slice i % slices of row a + i / slices, in order
+    const int lists = (b - a) * slices;
+    const float per_slice = 1.f / (float)slices;
+    const u64* mine = keys + (size_t)a * slices;     // (the lists' first candidates, then all second ones, ...)
+    const size_t all_lists = (size_t)rows * slices;
+    const int d = 1 << warp, n = (num + d - 1) / d;  // (see below) this warp's d
+    const bool looks = d <= num && n <= 32 && lists > 0;
+    constexpr int EARLY = 4;
+    u64 ahead[EARLY];                                // asked for before the rows' sums
 #pragma unroll
-        for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-        const double v = (double)scores[r] - ((double)m + log(sum));
-        if (lane == 0) { base[r] = isfinite(v) ? v : -(double)INFINITY; if (r - a < BASES) near_base[r - a] = base[r]; }
+    for (int e = 0; e < EARLY; ++e) ahead[e] = 0;
+    const u64* depth = mine + (d - 1) * all_lists;
+    const auto ask = [&](int i0) {                   // (a list twice behind the last one: no branch)
+#pragma unroll
+        for (int e = 0; e < EARLY; ++e) ahead[e] = depth[min(i0 + 32 * e, lists - 1)];
+    };
+    if (looks) ask(lane);
+    // s[r] - lse[r]: a warp per row, or a quarter of one
+    const int width = b - a > WARPS ? 8 : 32, part = threadIdx.x % width;
+    for (int r0 = a; r0 < b; r0 += NT / width) {
+        const int r = r0 + threadIdx.x / width;
+        const SliceSum* own = sums + (size_t)r * slices;
+        SliceSum all{0., -INFINITY, 1};
+        for (int i = part; i < slices && r < b; i += width) all = larger_unit(all, own[i]);
+        for (int o = width / 2; o > 0; o >>= 1) {
+            const SliceSum other{0., __shfl_xor_sync(0xffffffffu, all.at, o), __shfl_xor_sync(0xffffffffu, all.binary, o)};
+            all = larger_unit(all, other);
+        }
+        double sum = 0.;
+        if (all.at > -INFINITY)
+            for (int i = part; i < slices && r < b; i += width) sum += in_units(own[i], all);
+        for (int o = width / 2; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+        if (part == 0 && r < b) {
+            const double v = all.at > -INFINITY ? (double)scores[r] - (log_unit(all) + log(sum)) : NAN;
+            base[r] = isfinite(v) ? v : -(double)INFINITY;
+            if (r - a < BASES) near_base[r - a] = base[r];
+        }
     }
     if (threadIdx.x == 0) count = 0;
     __syncthreads();
-    // list i: row, slice; candidate k of it
-    const int lists = (b - a) * slices;
-    const auto at = [&](int list, int k) {
-        const int r = a + list / slices;
-        const size_t where = (size_t)r * slices + list % slices;
-        Candidate c{-(double)INFINITY, r, 0};
+    const auto candidate = [&](int list, u64 key) {
+        const int r = a + (int)(((float)list + 0.5f) * per_slice);      // list / slices: at most 65,535 lists, no rounding reaches the next whole number
         const double from = r - a < BASES ? near_base[r - a] : base[r];
-        if (k < num) c.key = keys[where * num + k];
-        if (c.key) c.value = from + (double)key_logit(c.key);
-        return c;
+        return Candidate{key ? from + (double)key_logit(key) : -(double)INFINITY, r, key};
     };
-    // A value that at least num candidates reach: from the heads where every warp has enough lists (list i belongs to warp i % 8), else the least of
-    // the depth-th candidates, depth the number of lists in num.
-    const int first = lane * WARPS + warp;
-    double least;
-    if (lists / WARPS >= turns(num)) {
-        double top = -(double)INFINITY;
-        for (int i = first; i < lists; i += NT) top = fmax(top, at(i, 0).value);
-        least = threshold(top, num, scratch);
-    } else {
-        const int depth = lists ? (num + lists - 1) / lists : 1;
-        double low = (double)INFINITY;
-        for (int i = first; i < lists; i += NT) low = fmin(low, at(i, depth - 1).value);
-        low = -warp_largest(-low);
-        if (lane == 0) scratch[warp] = low;
-        __syncthreads();
-        least = scratch[0];
-        for (int w = 1; w < WARPS; ++w) least = fmin(least, scratch[w]);
+    const auto at = [&](int list, int k) { return candidate(list, k < num ? mine[k * all_lists + list] : 0); };
+    // A value that at least num candidates reach: where n lists' d-th candidates reach it, n d candidates do.  Each warp takes another d, and of its 32 lanes (a lane
+    // has many lists) the ceil(num / d)-th best d-th candidate.  d = 1 is the good one where rows are alike, a large one where a row is far ahead.
+    {
+        float top = -INFINITY, nth = -INFINITY;
+        if (looks) {
+            for (int i = lane;;) {
+#pragma unroll
+                for (int e = 0; e < EARLY; ++e) {
+                    const int list = i + 32 * e;
+                    top = fmaxf(top, list < lists ? __double2float_rd(candidate(min(list, lists - 1), ahead[e]).value) : -INFINITY);
+                }
+                i += 32 * EARLY;
+                if (i - lane >= lists) break;
+                ask(i);
+            }
+            nth = warp_nth(top, n);
+        }
+        if (lane == 0) bounds[warp] = nth;
     }
+    __syncthreads();
+    double least = (double)bounds[0];
+#pragma unroll
+    for (int w = 1; w < WARPS; ++w) least = fmax(least, (double)bounds[w]);
+    // several threads to a list where there are few lists, four candidates at a time
+    const int step = lists ? max(1, NT / lists) : 1, skip = lists > NT ? NT : lists;
+    const int from = (int)threadIdx.x < step * skip ? threadIdx.x % skip : lists, k0 = skip ? threadIdx.x / skip : 0;
     int have;
     for (bool bounded = false;; bounded = true) {
-        for (int i = first; i < lists; i += NT)
-            for (int k = 0; k < num; ++k) {
-                const Candidate c = at(i, k);
-                if (!(c.value >= least && c.value > -(double)INFINITY) || (bounded && goes_before(bound, c))) break;      // lists are in order
-                const int p = atomicAdd(&count, 1);
-                if (p < CAP) found.put(p, c);
+        for (int i = from; i < lists; i += NT)
+            for (int k = k0, on = 1; k < num && on; k += 4 * step) {
+                Candidate c[4];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) c[e] = at(i, k + e * step);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    on = on && c[e].value >= least && c[e].value > -(double)INFINITY;      // lists are in order
+                    if (!on || (bounded && goes_before(bound, c[e]))) continue;
+                    const int p = atomicAdd(&count, 1);
+                    if (p < CAP) found.put(p, c[e]);
+                }
             }
         __syncthreads();
         have = count;
@@ -347,9 +501,11 @@ __global__ void __launch_bounds__(NT) beam_merge_kernel(const SliceSum* sums, co
     }
 }
 
-int slice_size(int rows, int vocab) {
-    // enough blocks for two an SM where the logits allow it
-    return (long long)rows * ((vocab + NT * 16 - 1) / (NT * 16)) >= 2ll * device_sms() ? 16 : 8;
+// Slices of a row: as many as give each block of a grid that fills the GPU once a share, of whole tiles.  shift: numbers between the row and the 16-byte boundary
+// in front of it, at most
+int slices_of(int rows, int vocab, int shift) {
+    const long long tiles = (vocab + (long long)shift + TILE - 1) / TILE, blocks = (long long)BLOCKS * device_sms() / (rows > 0 ? rows : 1), each = blocks > 0 ? (tiles + blocks - 1) / blocks : tiles;
+    return (int)((tiles + each - 1) / each);
 }
 
 }  // namespace
@@ -357,8 +513,7 @@ int slice_size(int rows, int vocab) {
 // Bytes of the work space of a call.
 MI_EXPORT long long mi_beam_select_bytes(int rows, int vocab, int num) {
     if (rows < 0 || vocab < 1 || num < 1 || num > MAX_NUM) return -2;
-    const int ept = slice_size(rows, vocab);
-    const long long slices = (vocab + (long long)NT * ept - 1) / (NT * ept);
+    const long long slices = std::max(slices_of(rows, vocab, 0), slices_of(rows, vocab, 3));
     return rows * (slices * (long long)(sizeof(SliceSum) + num * sizeof(u64)) + (long long)sizeof(double));
 }
 
@@ -368,15 +523,13 @@ MI_EXPORT int mi_beam_select(const float* logits, long long ld, int rows, int vo
                              float* values, int* chosen, void* work, cudaStream_t stream) {
     if (groups == 0) return 0;
     if (rows < 0 || groups < 0 || vocab < 1 || vocab > 0x7fffffff - NT * 32 || num < 1 || num > MAX_NUM || (rows && ld < vocab) || rows > 65535 || ((uintptr_t)work % 16)) return -2;
-    const int ept = slice_size(rows, vocab), slices = (vocab + NT * ept - 1) / (NT * ept);
+    const int shift = ((uintptr_t)logits | (uintptr_t)(ld * 4)) % 16 ? 3 : 0, slices = slices_of(rows, vocab, shift);
+    const int per = (int)(((long long)vocab + shift + slices - 1) / slices + 3) / 4 * 4;
     SliceSum* sums = (SliceSum*)work;
     u64* keys = (u64*)(sums + (size_t)rows * slices);
     double* base = (double*)(keys + (size_t)rows * slices * num);
     if (rows) {
-        cudaError_t e;
-        const dim3 grid(slices, rows);
-        if (ept == 16) e = launch_pdl(beam_slice_kernel<16>, grid, dim3(NT), 0, stream, logits, ld, vocab, num, sums, keys);
-        else e = launch_pdl(beam_slice_kernel<8>, grid, dim3(NT), 0, stream, logits, ld, vocab, num, sums, keys);
+        const cudaError_t e = launch_pdl(beam_slice_kernel, dim3(slices, rows), dim3(NT), AHEAD * TILE * 4, stream, logits, ld, vocab, per, num, sums, keys);
         if (e != cudaSuccess) return (int)e;
     }
     return (int)launch_pdl(beam_merge_kernel, dim3(groups), dim3(NT), 0, stream, sums, keys, slices, num, scores, rows, group_start, base, values, chosen,
