@@ -93,6 +93,27 @@ def test_beam_select_wide_range(ops):
 
 
 @gpu
+def test_beam_select_along_long_rows(ops):
+    """So many rows that a block streams several tiles: logits that rise or fall along them, past a thousand and back, begin with nothing, or are all the same."""
+    R, V = 300, 20003
+    x, s = model_logits(R, V, seed=21)
+    along = torch.linspace(0, 1, V)
+    x[0:20] += along * 30
+    x[20:40] -= along * 60
+    x[40:60] += along * 3000 - 1500                              # below a thousand, then above
+    x[60:80] -= along * 3000 - 1500
+    x[80:100, :9001] = -math.inf
+    x[100:120, 9001:] = -math.inf
+    x[120:140] = 0.5
+    x[140:150, ::2] = -math.inf
+    x[150, 19000], x[151, 2] = math.nan, math.inf
+    x[152:160] = x[152:160].round()
+    x[160:170] += (torch.arange(V) % 8192 // 4096) * 2000        # up and down by turns
+    check_select(ops, x, s, (100, 20, 20, 30, 130), 24)
+    check_select(ops, x, s, (150, 150), 128)
+
+
+@gpu
 def test_beam_select_strides_streams_and_graphs(ops):
     x, s = model_logits(6, 10007, seed=4)
     wide = torch.full((6, 10050), math.nan, device=DEV)
