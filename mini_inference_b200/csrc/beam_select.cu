@@ -517,10 +517,10 @@ MI_EXPORT long long mi_beam_select_bytes(int rows, int vocab, int num) {
     return rows * (slices * (long long)(sizeof(SliceSum) + num * sizeof(u64)) + (long long)sizeof(double));
 }
 
-// logits float32 [rows, vocab], rows ld apart; scores float32 [rows]; group_start int32 [groups + 1]; values float32 [groups, num], chosen int32 [2, groups, num]: rows, then tokens.
+// logits float32 [rows, vocab], rows ld apart; scores float32 [rows]; group_start int32 [groups + 1]; values float32, chosen_rows and chosen_tokens int32 [groups, num].
 // work: mi_beam_select_bytes of it, on 16 bytes.
 MI_EXPORT int mi_beam_select(const float* logits, long long ld, int rows, int vocab, const float* scores, const int* group_start, int groups, int num,
-                             float* values, int* chosen, void* work, cudaStream_t stream) {
+                             float* values, int* chosen_rows, int* chosen_tokens, void* work, cudaStream_t stream) {
     if (groups == 0) return 0;
     if (rows < 0 || groups < 0 || vocab < 1 || vocab > 0x7fffffff - NT * 32 || num < 1 || num > MAX_NUM || (rows && ld < vocab) || rows > 65535 || ((uintptr_t)work % 16)) return -2;
     const int shift = ((uintptr_t)logits | (uintptr_t)(ld * 4)) % 16 ? 3 : 0, slices = slices_of(rows, vocab, shift);
@@ -532,6 +532,6 @@ MI_EXPORT int mi_beam_select(const float* logits, long long ld, int rows, int vo
         const cudaError_t e = launch_pdl(beam_slice_kernel, dim3(slices, rows), dim3(NT), AHEAD * TILE * 4, stream, logits, ld, vocab, per, num, sums, keys);
         if (e != cudaSuccess) return (int)e;
     }
-    return (int)launch_pdl(beam_merge_kernel, dim3(groups), dim3(NT), 0, stream, sums, keys, slices, num, scores, rows, group_start, base, values, chosen,
-                           chosen + (size_t)groups * num);
+    return (int)launch_pdl(beam_merge_kernel, dim3(groups), dim3(NT), 0, stream, sums, keys, slices, num, scores, rows, group_start, base, values, chosen_rows,
+                           chosen_tokens);
 }

@@ -715,7 +715,7 @@ class CudaOps:
                                           page_size=meta.page_size, block_table=meta.block_table, table_rows=getattr(meta, "table_rows", None), shared_start=None,
                                           decode_segs=meta.decode_segs, seg_q_start=meta.seg_q_start, seg_kv_len=meta.seg_kv_len)
             return self.paged_attention(q, k_cache, v_cache, alone, H, KV, D, scale, None)
-        out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+        out = torch.empty_like(q, memory_format=torch.contiguous_format)
         self._shared_decode(q, k_cache, v_cache, out, meta, H, KV, D, scale, size)
         return out
 
@@ -727,9 +727,9 @@ class CudaOps:
         return size(meta.decode_segs.shape[0], meta.shared_len.shape[0], meta.max_shared_rows, H, KV, D, meta.page_size)
 
     def _shared_decode(self, q, k_cache, v_cache, out, meta, H, KV, D, scale, size):
-        work = torch.empty(size, dtype=torch.uint8, device=q.device)
-        rows = (out, meta.decode_segs, meta.decode_segs.shape[0], meta.seg_q_start, meta.seg_kv_len, meta.seg_kv_len.shape[0], meta.block_table, getattr(meta, "table_rows", None), meta.max_pages,
-                meta.shared_start, meta.shared_len, meta.shared_len.shape[0], meta.max_shared_rows, H, KV, D, meta.page_size, scale, work)
+        segs, kv_len, shared = meta.decode_segs, meta.seg_kv_len, meta.shared_len
+        rows = (out, segs, len(segs), meta.seg_q_start, kv_len, len(kv_len), meta.block_table, getattr(meta, "table_rows", None), meta.max_pages, meta.shared_start,
+                shared, len(shared), meta.max_shared_rows, H, KV, D, meta.page_size, scale, segs.new_empty((size + 3) // 4))
         if q.dtype is torch.bfloat16:
             _check(self.lib.mi_attn_shared_tc(q, q.stride(0), q.shape[0], k_cache, v_cache, k_cache.shape[0] * KV * meta.page_size, *rows, self._stream_error, self._stream()),
                    "attn_shared_tc")
@@ -1823,16 +1823,14 @@ class CudaOps:
         if self._elsewhere():
             with torch.cuda.device(here):
                 return self.beam_select(logits, scores, group_start, num)
-        dev = logits.device
-        values = torch.empty((G, num), dtype=torch.float32, device=dev)
-        chosen = torch.empty((2, G, num), dtype=torch.int32, device=dev)
         n = self.lib.mi_beam_select_bytes(R, V, num)
         if n < 0:
             _check(n, "beam_select")
-        work = torch.empty(n, dtype=torch.uint8, device=dev)
-        _check(self.lib.mi_beam_select(logits, ld if R > 1 else V, R, V, scores, group_start, G, num, values, chosen, work, self._stream()), "beam_select")
+        values, rows, work = scores.new_empty((G, num)), group_start.new_empty((G, num)), group_start.new_empty((n + 3) // 4)
+        tokens = torch.empty_like(rows)
+        _check(self.lib.mi_beam_select(logits, ld if R > 1 else V, R, V, scores, group_start, G, num, values, rows, tokens, work, self._stream()), "beam_select")
         self.launches += (2 if R else 1) if G else 0
-        return values, *chosen.unbind()
+        return values, rows, tokens
 
     def _refuse_select(self, logits, scores, group_start, num):
         """Raises what is wrong with a call of beam_select."""
