@@ -160,12 +160,13 @@ __global__ void attn_decode_merge_kernel(const float* __restrict__ o_part, const
     const size_t base = ((size_t)i * H + h) * S;
     float mx = -INFINITY;
     for (int s = 0; s < S; ++s) mx = fmaxf(mx, lse_part[base + s]);
+    if (mx == -INFINITY) mx = 0.f;                              // an entry without keys: output 0
     float den = 0.f;
     for (int s = 0; s < S; ++s) den += expf(lse_part[base + s] - mx);
     for (int d = threadIdx.x; d < D; d += blockDim.x) {
         float num = 0.f;
         for (int s = 0; s < S; ++s) num += expf(lse_part[base + s] - mx) * o_part[(base + s) * D + d];
-        out[((size_t)tok * H + h) * D + d] = from_f32<T>(num / den);
+        out[((size_t)tok * H + h) * D + d] = from_f32<T>(den == 0.f ? 0.f : num / den);
     }
 }
 

@@ -174,6 +174,7 @@ int slot_rows_of(int H, int KV, int most) { const int t = tile_rows_of(H, KV); r
 // Bytes of the work space of a call; -2: sizes that this kernel does not take.  most: rows of the largest group.
 MI_EXPORT long long mi_attn_shared_f32_bytes(int R, int G, int most, int H, int KV, int D, int ps) {
     if (!fits(R, G, H, KV, D, ps)) return -2;
+    most = most > R ? R : most;
     return scratch(R, G, KV, D, row_tiles_of(H, KV, most), slot_rows_of(H, KV, most), H / KV, 2 * device_sms()).bytes;
 }
 
@@ -185,6 +186,7 @@ MI_EXPORT int mi_attn_shared_f32(const float* q, int q_stride, const float* k_ca
     if (R == 0) return 0;
     if (!fits(R, G, H, KV, D, ps) || entries < 1 || q_stride % 4 || (((uintptr_t)q | (uintptr_t)k_cache | (uintptr_t)v_cache | (uintptr_t)work) % 16)) return -2;
     const int blocks = 2 * device_sms();
+    most = most > R ? R : most;
     Args a{decode_segs, seg_q_start, seg_kv_len, block_table, table_rows, shared_start, shared_len, R, G, entries, most > 1 ? most : 1, table_stride, H, KV, ps,
            row_tiles_of(H, KV, most), tile_rows_of(H, KV), 0, slot_rows_of(H, KV, most), H / KV};
     place_scratch(a, scratch(R, G, KV, D, a.row_tiles, a.slot_rows, a.tail_rows, blocks), work);

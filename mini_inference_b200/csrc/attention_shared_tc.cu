@@ -430,6 +430,7 @@ int tail_rows_of(int H, int KV) { return copies_of(1, H / KV) * (H / KV); }
 // Bytes of the work space of a call; -2: sizes that this kernel does not take.  most: rows of the largest group.
 MI_EXPORT long long mi_attn_shared_tc_bytes(int R, int G, int most, int H, int KV, int D, int ps) {
     if (!fits(R, G, H, KV, D, ps)) return -2;
+    most = most > R ? R : most;
     return scratch(R, G, KV, D, row_tiles_of(H, KV, most), slot_rows_of(H, KV, most), tail_rows_of(H, KV), 2 * device_sms()).bytes;
 }
 
@@ -445,6 +446,7 @@ MI_EXPORT int mi_attn_shared_tc(const void* q, int q_stride, int tokens, const v
     if (!query_map(q, tokens, H, D, q_stride, H / KV, &qmap)) return -5;
     if (!cache_map(k_cache, cache_rows, D, ps < KT ? ps : KT, &kmap) || !cache_map(v_cache, cache_rows, D, ps < KT ? ps : KT, &vmap)) return -5;
     const int blocks = 2 * device_sms();
+    most = most > R ? R : most;
     Args a{decode_segs, seg_q_start, seg_kv_len, block_table, table_rows, shared_start, shared_len, R, G, entries, most > 1 ? most : 1, table_stride, H, KV, ps,
            row_tiles_of(H, KV, most), tile_rows_of(H, KV), 1, slot_rows_of(H, KV, most), tail_rows_of(H, KV)};
     place_scratch(a, scratch(R, G, KV, D, a.row_tiles, a.slot_rows, a.tail_rows, blocks), work);

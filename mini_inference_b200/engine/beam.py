@@ -31,8 +31,8 @@ class BeamParams:
             raise ValueError(f"{self.num_beams} beams: between 1 and {MAX_BEAMS} are possible")
         if self.max_new_tokens < 1:
             raise ValueError("max_new_tokens must be positive")
-        if not math.isfinite(self.length_penalty):
-            raise ValueError("length_penalty must be a finite number")
+        if not abs(self.length_penalty) <= 64:            # (a length to that power is still a float)
+            raise ValueError("length_penalty must be between -64 and 64")
 
 
 @dataclass

@@ -618,7 +618,7 @@ class CudaOps:
             self.launches += 1
         if not num_decode:
             return out
-        if not win and not split_weights and getattr(meta, "shared_start", None) is not None:
+        if not win and not split_weights and getattr(meta, "shared_start", None) is not None and self._sharing_pays(q, meta, KV, D, q.dtype is torch.bfloat16):
             size = self._shared_bytes(q, k_cache, v_cache, meta, H, KV, D)
             if size > 0:
                 self._shared_decode(q, k_cache, v_cache, out, meta, H, KV, D, scale, size)
@@ -667,7 +667,7 @@ class CudaOps:
         same, and are read by the pages of the first row that has them all; max_shared_rows, on the host: rows of the largest group (rows beyond it are computed alone).  An entry
         without keys gets zeros.  The output [T, H D] has the entries' rows; others are left as they come.
         Heads of 64 or 128 run on kernels that share; other heads, more than 4,096 entries and groups, bfloat16 pages that neither divide 64 keys nor are divided
-        by them, and bfloat16 rows that do not lie whole heads apart are computed row by row, by the rows' own pages."""
+        by them, bfloat16 rows that do not lie whole heads apart, and float32 caches that are small (SHARED_BYTES) are computed row by row, by the rows' own pages."""
         rows = getattr(meta, "table_rows", None)
         lists = (meta.decode_segs, meta.seg_q_start, meta.seg_kv_len, meta.shared_start, meta.shared_len)
         tables = (meta.block_table,) if rows is None else (meta.block_table, rows)
@@ -709,19 +709,42 @@ class CudaOps:
         if self._elsewhere():
             with torch.cuda.device(self._device_index):
                 return self._shared_or_alone(q, k_cache, v_cache, meta, H, KV, D, scale)
-        size = self._shared_bytes(q, k_cache, v_cache, meta, H, KV, D)
-        if size <= 0:
-            alone = types.SimpleNamespace(prefill_tiles=meta.decode_segs[:0].view(0, 2), tile=self.prefill_tile, max_kv_len=meta.max_kv_len, max_pages=meta.max_pages,
-                                          page_size=meta.page_size, block_table=meta.block_table, table_rows=getattr(meta, "table_rows", None), shared_start=None,
-                                          decode_segs=meta.decode_segs, seg_q_start=meta.seg_q_start, seg_kv_len=meta.seg_kv_len)
-            return self.paged_attention(q, k_cache, v_cache, alone, H, KV, D, scale, None)
         out = torch.empty_like(q, memory_format=torch.contiguous_format)
-        self._shared_decode(q, k_cache, v_cache, out, meta, H, KV, D, scale, size)
+        size = self._shared_bytes(q, k_cache, v_cache, meta, H, KV, D) if q.dtype is torch.bfloat16 or self._sharing_pays(q, meta, KV, D, False) else 0
+        if size > 0:
+            self._shared_decode(q, k_cache, v_cache, out, meta, H, KV, D, scale, size)
+        else:
+            self._decode_alone(q, k_cache, v_cache, out, meta, H, KV, D, scale)
         return out
+
+    def _decode_alone(self, q, k_cache, v_cache, out, meta, H, KV, D, scale):
+        """Entries one by one, each by its own pages, on the kernels that read nothing behind an entry's keys and keep nothing between calls."""
+        if (k_cache.data_ptr() | v_cache.data_ptr()) % 16:
+            raise ValueError("shared_prefix_attention: caches that do not start on 16 bytes")
+        n = len(meta.decode_segs)
+        S = self.choose_splits(n * math.ceil(H / 4), meta.max_kv_len)
+        o_part = lse = None
+        if S > 1:
+            o_part, lse = (torch.empty(shape, dtype=torch.float32, device=q.device) for shape in ((n, H, S, D), (n, H, S)))
+        _check(self.lib.mi_attn_decode_generic(q, q.stride(0), k_cache, v_cache, out, o_part, lse, meta.decode_segs, n, meta.seg_q_start, meta.seg_kv_len, meta.block_table,
+                                               getattr(meta, "table_rows", None), meta.max_pages, H, KV, D, meta.page_size, S, scale, 0, _code(q.dtype), self._stream()), "attn_decode")
+        self.launches += 2 if S > 1 else 1
+
+    # What the rows would read one by one, from which on sharing is the faster way: less stays in the L2 cache from one row to the next.  Microseconds, sharing / one by one, 32
+    # heads over 8 of 128.  bfloat16 (paged_attention's decode kernel): 4 rows x 512 keys 15 / 8, 8 x 4,096 (135 MB) 25 / 24, 16 x 2,048 (136 MB) 19 / 24, 4 groups of
+    # 8 x 1,024 (138 MB) 24 / 22, 8 x 8 x 1,024 (277 MB) 30 / 44, 8 x 8 x 4,096 46 / 146.  float32, whose multiply-adds bound the shared form: 13 rows x 1,600 (171 MB) 37 / 31,
+    # 8 x 4,096 (270 MB) 44 / 44, 8 x 8 x 512 (285 MB) 75 / 49, 16 x 4,096 (541 MB) 68 / 78, 8 x 16 x 512 (570 MB) 126 / 97, 8 x 8 x 2,048 (1.1 GB) 137 / 175.
+    # (shared_prefix_attention itself shares bfloat16 at every size: that decode kernel wants finite numbers in the unused ends of pages, a key per entry, and its counters to itself.)
+    SHARED_BYTES = {torch.bfloat16: 128 << 20, torch.float32: 512 << 20}
+
+    def _sharing_pays(self, q, meta, KV, D, bf16):
+        return len(meta.decode_segs) * meta.max_kv_len * KV * D * (4 if bf16 else 8) > self.SHARED_BYTES[q.dtype]
 
     def _shared_bytes(self, q, k_cache, v_cache, meta, H, KV, D):
         """Bytes of scratch of the kernel that reads shared prefixes once; not above 0: these rows are computed one by one."""
-        if not self.fast_attention or q.stride(0) % (D if q.dtype is torch.bfloat16 else 4) or (q.data_ptr() | k_cache.data_ptr() | v_cache.data_ptr()) % 16:
+        stride = q.stride(0) if len(q) > 1 else H * D
+        if (not self.fast_attention or stride % (D if q.dtype is torch.bfloat16 else 4) or stride < H * D
+                or (q.data_ptr() | k_cache.data_ptr() | v_cache.data_ptr()) % 16):
             return 0
         size = self.lib.mi_attn_shared_tc_bytes if q.dtype is torch.bfloat16 else self.lib.mi_attn_shared_f32_bytes
         return size(meta.decode_segs.shape[0], meta.shared_len.shape[0], meta.max_shared_rows, H, KV, D, meta.page_size)
@@ -731,7 +754,7 @@ class CudaOps:
         rows = (out, segs, len(segs), meta.seg_q_start, kv_len, len(kv_len), meta.block_table, getattr(meta, "table_rows", None), meta.max_pages, meta.shared_start,
                 shared, len(shared), meta.max_shared_rows, H, KV, D, meta.page_size, scale, segs.new_empty((size + 3) // 4))
         if q.dtype is torch.bfloat16:
-            _check(self.lib.mi_attn_shared_tc(q, q.stride(0), q.shape[0], k_cache, v_cache, k_cache.shape[0] * KV * meta.page_size, *rows, self._stream_error, self._stream()),
+            _check(self.lib.mi_attn_shared_tc(q, q.stride(0) if len(q) > 1 else H * D, len(q), k_cache, v_cache, k_cache.shape[0] * KV * meta.page_size, *rows, self._stream_error, self._stream()),
                    "attn_shared_tc")
         else:
             _check(self.lib.mi_attn_shared_f32(q, q.stride(0), k_cache, v_cache, *rows, self._stream()), "attn_shared_f32")
@@ -1848,9 +1871,11 @@ class CudaOps:
         """In place, for every tensor t of `tensors` and every i: t[rows[i]] = what t[rows[parents[i]]] was before the call (a beam takes over its parent's
         state).  dim: which dimension of the tensors the rows are (those before it are as many tables with the same rows; tensors of any type, contiguous
         from the rows' dimension on, and before it too).  rows, parents int32 [n]; group_start int32 [G + 1]: places group_start[g] .. group_start[g + 1] - 1 of
-        both lists are a group, parents (places in the lists) lie in their row's group; most: rows of the largest group, at most 100.  A row is named once.
-        A parent outside its group, or a row that a tensor does not have, leaves the row as it is."""
+        both lists are a group, parents (places in the lists) lie in their row's group; most: rows of the largest group, at most 100.  A row is named once, no
+        tensor twice.  A parent outside its group, or a row that a tensor does not have, leaves the row as it is."""
         tensors, here = list(tensors), self._device_index
+        if len(set(map(torch.Tensor.data_ptr, tensors))) < len(tensors) and len({t.data_ptr() for t in tensors if t.numel()}) < sum(t.numel() > 0 for t in tensors):
+            raise ValueError("reorder_rows: two of the tensors are the same memory")
         if (not (rows.dtype is parents.dtype is group_start.dtype is torch.int32) or not (rows.is_contiguous() and parents.is_contiguous() and group_start.is_contiguous())
                 or rows.dim() != 1 or rows.shape != parents.shape or group_start.dim() != 1 or group_start.shape[0] < 1 or not 0 <= most <= self.MAX_BEAMS):
             self._plain("reorder_rows", torch.int32, rows=rows, parents=parents, group_start=group_start)

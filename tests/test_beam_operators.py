@@ -277,6 +277,15 @@ def test_reorder_rows_refuses():
             me.reorder_rows(*args, **kw)
 
 
+def test_reorder_rows_refuses_a_tensor_twice():
+    me, t, rows, start = bare(), torch.zeros(6, 3, 4), torch.arange(4, dtype=torch.int32), starts((4,))
+    for tensors in ([t, t], [t, torch.zeros(6, 1), t.view(6, 12)]):
+        with pytest.raises(ValueError, match="same memory"):
+            me.reorder_rows(tensors, rows, rows, start, 4)
+    with pytest.raises(ValueError, match="cuda:0"):               # empty ones have no memory
+        me.reorder_rows([t, torch.zeros(0, 3), torch.zeros(0, 5)], rows, rows, start, 4)
+
+
 def test_reorder_plain_statement():
     """Every row gets what its parent held before the call, whatever the order."""
     t = torch.arange(6.0).view(6, 1)

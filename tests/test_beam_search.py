@@ -153,7 +153,7 @@ def test_greedy_is_one_beam(tiny_dirs):
 def test_refusals(tiny_dirs):
     d, cfg, page = tiny_dirs["A"]
     llm = engine(d, page, "cpu", max_num_seqs=4, kv_cache_tokens=page * 8, kv_watermark=0.0)
-    for bad in (dict(num_beams=0), dict(num_beams=65), dict(max_new_tokens=0), dict(length_penalty=math.nan), dict(length_penalty=math.inf)):
+    for bad in (dict(num_beams=0), dict(num_beams=65), dict(max_new_tokens=0), dict(length_penalty=math.nan), dict(length_penalty=math.inf), dict(length_penalty=65.0), dict(length_penalty=-1e9)):
         with pytest.raises(ValueError):
             BeamParams(**bad)
     with pytest.raises(ValueError, match="holds 4 sequences"):

@@ -5,6 +5,7 @@ import types
 import pytest
 import torch
 
+from mini_inference_b200.ops import CudaOps
 from tests.ref_beam import shared_prefix_attention64
 from tests.test_beam_operators import bare, starts
 
@@ -73,6 +74,13 @@ def problem(groups, H, KV, D, ps, dtype, seed=0, alone=(), garbage=math.nan, ext
                                  shared_len=i32([s for s, _ in groups]), max_shared_rows=max([len(ns) for _, ns in groups] + [0]))
     q = torch.randn(q_start[-1], (H + 2 * KV) * D, generator=g).to(dtype).to(DEV)[:, :H * D]
     return q, k.to(dtype).to(DEV), v.to(dtype).to(DEV), meta
+
+
+@pytest.fixture(params=["by the rule", "shared at any size"], autouse=True)
+def form(request, monkeypatch):
+    """Small float32 caches go to the kernel without sharing; every test runs on both."""
+    if request.param != "by the rule":
+        monkeypatch.setattr(CudaOps, "SHARED_BYTES", {BF16: 0, F32: 0})
 
 
 def check(ops, q, k, v, meta, H, KV, D, scale=None, got=None):
@@ -235,6 +243,41 @@ def test_as_many_entries_as_it_takes(ops):
         q, k, v, meta = problem([(16, [17, 18, 19, 20])] * n, 4, 1, 64, 16, BF16, seed=12, garbage=math.nan if takes else 0.0)
         assert (ops._shared_bytes(q, k, v, meta, 4, 1, 64) > 0) == takes
         check(ops, q, k, v, meta, 4, 1, 64)
+
+
+@gpu
+@pytest.mark.parametrize("H,KV,D,ps,dtype", [(6, 3, 48, 4, BF16), (6, 3, 32, 4, F32), (10, 2, 128, 32, F32), (8, 2, 64, 16, F32)])
+def test_entries_without_keys_computed_alone(ops, H, KV, D, ps, dtype, monkeypatch):
+    """Zeros, in one piece and where the longest entry makes several, and nothing of what lies behind the keys."""
+    monkeypatch.setattr(CudaOps, "SHARED_BYTES", {BF16: 0, F32: 1 << 60})
+    for groups in (GROUPS["no keys"], [(0, [0, 3000, 1]), (700, [700, 0, 701])]):
+        q, k, v, meta = problem(groups, H, KV, D, ps, dtype, seed=13)
+        check(ops, q, k, v, meta, H, KV, D)
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [BF16, F32])
+def test_query_rows_of_any_stride_and_more_rows_than_there_are(ops, dtype):
+    H, KV, D = 8, 2, 128
+    q, k, v, meta = problem(GROUPS["four beams"], H, KV, D, 16, dtype, seed=14)
+    meta.max_shared_rows = 2 ** 31 - 1
+    check(ops, q, k, v, meta, H, KV, D)
+    check(ops, q[:1].expand(4, -1), k, v, meta, H, KV, D)          # all rows the same memory
+    wide = torch.randn(4, H * D + 4, device=DEV).to(dtype)
+    check(ops, wide[:, :H * D], k, v, meta, H, KV, D)              # rows that do not lie whole heads apart
+    q, k, v, meta = problem(GROUPS["one beam"], H, KV, D, 16, dtype, seed=15)
+    check(ops, torch.randn(3, H * D + 8, device=DEV).to(dtype)[1:2, 8:], k, v, meta, H, KV, D)
+    check(ops, q.contiguous().as_strided((1, H * D), (0, 1)), k, v, meta, H, KV, D)
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [BF16, F32])
+def test_caches_off_16_bytes_are_refused(ops, dtype):
+    q, k, v, meta = problem(GROUPS["short"], 8, 2, 128, 16, dtype, seed=16)
+    off = torch.zeros(k.numel() + 1, dtype=dtype, device=DEV)[1:].view(k.shape)
+    for caches in ((off, v), (k, off)):
+        with pytest.raises(ValueError, match="16 bytes"):
+            ops.shared_prefix_attention(q, *caches, meta, 8, 2, 128, 0.1)
 
 
 def test_refusals():
