@@ -80,7 +80,8 @@ constexpr int DEC_WARPS_ALONE = 8; // warps of a block that has its SM to itself
 // (16 mantissa bits in all, summed in float32), for designs that want their attention weights in more than 16-bit precision.
 // EXT: the scaled score s becomes cap * tanh(s / cap) (cap > 0), the first `keep` keys of a request stay visible whatever the window,
 // and the output is multiplied by sigmoid(gate), gate bfloat16 [T, H D] with rows gate_stride apart (null: no gate).
-struct DecodeExt { float cap; int keep; const __nv_bfloat16* gate; int gate_stride; };
+// careful: nothing is read before the kernel ahead is done (it may have written any page or list), and splits that do not merge as a cluster are not made.
+struct DecodeExt { float cap; int keep; const __nv_bfloat16* gate; int gate_stride; int careful; };
 
 template <int D, bool BULK, int WARPS, bool SPLIT = false, bool BIAS = false, bool EXT = false>
 __global__ void __launch_bounds__(WARPS * 32, WARPS > DEC_WARPS ? 1 : BULK ? 2 : 3)
@@ -107,7 +108,7 @@ attn_decode_mma_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_co
     extern __shared__ float smem_raw[];  // [WARPS][16][D] outputs, then [WARPS][16] max and sum
     float* smem = smem_raw;
     pdl_trigger();
-    if (!BULK) pdl_wait(q, k_cache, v_cache);
+    if (!BULK || ext.careful) pdl_wait(q, k_cache, v_cache);
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int g = lane >> 2, c = lane & 3;
     const int G = H / KV;
@@ -332,6 +333,14 @@ attn_decode_mma_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_co
                 pr[2] = pack_bf16(p[1][0], p[1][1]); pr[3] = pack_bf16(p[1][2], p[1][3]);
             }
         }
+        // values behind the last key may be anything (the unused end of a page), and 0 * inf is no 0
+        if (blk_of(blk) * 16 + 16 > len) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                if (blk_of(blk) * 16 + 2 * c + (i & 1) + 8 * (i >> 1) >= len)
+#pragma unroll
+                    for (int hb = 0; hb < HALVES; ++hb) vreg[i][hb] = make_uint4(0, 0, 0, 0);
+        }
         // O += P V; tile t of half hb: column g is d = 64 hb + 8 g + t
 #pragma unroll
         for (int hb = 0; hb < HALVES; ++hb) {
@@ -413,6 +422,7 @@ attn_decode_mma_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_co
                     v[r] = r < S ? ld_cluster(cpart + idx, r) : 0.f;
                     mx = fmaxf(mx, l[r]);
                 }
+                if (mx == -INFINITY) mx = 0.f;                 // an entry without keys: output 0
                 float num = 0.f, den = 0.f;
 #pragma unroll
                 for (int r = 0; r < 8; ++r) {
@@ -420,7 +430,7 @@ attn_decode_mma_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_co
                     den += w;
                     num += w * v[r];
                 }
-                out[((size_t)tok * H + h) * D + d] = __float2bfloat16_rn(gated(num / den, h, d));
+                out[((size_t)tok * H + h) * D + d] = __float2bfloat16_rn(gated(den == 0.f ? 0.f : num / den, h, d));
             }
         }
         cluster_sync();                                    // the others' shared memory stays until split 0 has read it
@@ -448,6 +458,7 @@ attn_decode_mma_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_co
 #pragma unroll
             for (int j = 0; j < 8; ++j) mx = fmaxf(mx, l[j]);
         }
+        if (mx == -INFINITY) mx = 0.f;
         for (int k0 = 0; k0 < S; k0 += 8) {
             float l[8], v[8];
 #pragma unroll
@@ -463,7 +474,7 @@ attn_decode_mma_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_co
                 num += w * v[j];
             }
         }
-        out[((size_t)tok * H + h) * D + d] = __float2bfloat16_rn(gated(num / den, h, d));
+        out[((size_t)tok * H + h) * D + d] = __float2bfloat16_rn(gated(den == 0.f ? 0.f : num / den, h, d));
     }
     if (threadIdx.x == 0) merge_counters[blockIdx.x * KV + kvh] = 0;       // ready for the next call
 }
@@ -574,7 +585,7 @@ static int decode_mma_rows_launch(const void* q, int q_stride, const void* k_cac
                                   float scale, int window, int* merge_counters, int* error_word, int cache_pages,
                                   int cluster_merge, cudaStream_t stream, int block = 0, int sink = 0,
                                   const float* sink_values = nullptr, const float* bias_t = nullptr, int bias_last = 0,
-                                  const float* slopes = nullptr, const DecodeExt& ext = DecodeExt{0.f, 0, nullptr, 0}) {
+                                  const float* slopes = nullptr, const DecodeExt& ext = DecodeExt{0.f, 0, nullptr, 0, 0}) {
     if (num_decode == 0) return 0;
     if ((D != 64 && D != 128) || H % KV || H / KV > 16 || ps % 16 || q_stride % 8) return -2;
     dim3 grid(num_decode, KV, splits);
@@ -593,14 +604,13 @@ static int decode_mma_rows_launch(const void* q, int q_stride, const void* k_cac
         if (cudaGetDevice(&dev) != cudaSuccess || cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess) sms = 1;
     }
     const bool alone = bulk && (long long)num_decode * KV * splits <= sms;      // at most one block per SM
-    const int warps = alone ? DEC_WARPS_ALONE : DEC_WARPS;
-    const size_t merge_bytes = (size_t)warps * 16 * (D + 2) * sizeof(float);
-    const size_t ring_bytes = bulk ? (size_t)warps * DEC_STAGES * 2 * 16 * D * 2 : 0;
-    const size_t smem = (ring_bytes > merge_bytes ? ring_bytes : merge_bytes) + (size_t)(D / 16) * 32 * 16 + warps * DEC_STAGES * 8 +
-                        (bulk ? 1024 + DEC_BAR_BYTES : 0);
     const float scale_log2 = scale * 1.4426950408889634f;
-    int use_cluster = (error_word != nullptr && cluster_merge && splits >= 2 && splits <= 8) ? 1 : 0;
 #define LAUNCH(DD, BB, WW) do { \
+        const size_t merge_bytes = (size_t)WW * 16 * (D + 2) * sizeof(float); \
+        const size_t ring_bytes = bulk ? (size_t)WW * DEC_STAGES * 2 * 16 * D * 2 : 0; \
+        const size_t smem = (ring_bytes > merge_bytes ? ring_bytes : merge_bytes) + (size_t)(D / 16) * 32 * 16 + WW * DEC_STAGES * 8 + \
+                            (bulk ? 1024 + DEC_BAR_BYTES : 0); \
+        int use_cluster = (error_word != nullptr && cluster_merge && splits >= 2 && splits <= 8) ? 1 : 0; \
         static bool configured = false; \
         if (!configured && smem > 48 * 1024) { \
             cudaError_t e = cudaFuncSetAttribute(attn_decode_mma_kernel<DD, BB, WW, SPLIT, BIAS, EXT>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem); \
@@ -627,13 +637,17 @@ static int decode_mma_rows_launch(const void* q, int q_stride, const void* k_cac
             /* (with a margin: blocks of the kernels before and after share the SMs for a moment) */ \
             if (fit[splits] < 0 || (long long)num_decode * KV * 100 > (long long)fit[splits] * 92) use_cluster = 0; \
         } \
+        if (ext.careful && !use_cluster) { \
+            if (splits > 1 && WW != DEC_WARPS) break;          /* the smaller block's clusters may fit */ \
+            cfg.gridDim.z = 1; \
+        } \
         cfg.attrs = use_cluster ? attr : attr + 1; cfg.numAttrs = use_cluster ? 2 : 1; \
         return (int)cudaLaunchKernelEx(&cfg, attn_decode_mma_kernel<DD, BB, WW, SPLIT, BIAS, EXT>, kmap, vmap, \
             (const __nv_bfloat16*)q, q_stride, (const __nv_bfloat16*)k_cache, (const __nv_bfloat16*)v_cache, \
             (__nv_bfloat16*)out, o_part, lse_part, decode_segs, seg_q_start, seg_kv_len, block_table, table_rows, \
             table_stride, H, KV, ps, scale_log2, window, merge_counters, error_word, use_cluster, block, sink, sink_values, bias_t, bias_last, slopes, ext); } while (0)
-    if (D == 128) { if (alone) LAUNCH(128, true, DEC_WARPS_ALONE); else if (bulk) LAUNCH(128, true, DEC_WARPS); else LAUNCH(128, false, DEC_WARPS); }
-    else { if (alone) LAUNCH(64, true, DEC_WARPS_ALONE); else if (bulk) LAUNCH(64, true, DEC_WARPS); else LAUNCH(64, false, DEC_WARPS); }
+    if (D == 128) { if (alone) LAUNCH(128, true, DEC_WARPS_ALONE); if (bulk) LAUNCH(128, true, DEC_WARPS); else LAUNCH(128, false, DEC_WARPS); }
+    else { if (alone) LAUNCH(64, true, DEC_WARPS_ALONE); if (bulk) LAUNCH(64, true, DEC_WARPS); else LAUNCH(64, false, DEC_WARPS); }
 #undef LAUNCH
     return (int)cudaGetLastError();
 }
@@ -647,6 +661,17 @@ MI_EXPORT int mi_attn_decode_mma_rows(const void* q, int q_stride, const void* k
                                       float scale, int window, int* merge_counters, int* error_word, int cache_pages,
                                       int cluster_merge, cudaStream_t stream) {
     return decode_mma_rows_launch<false>(DECODE_ROWS_ARGS);
+}
+
+// The same for a caller that may come directly behind a kernel that writes pages or lists, beside another call on another stream: the splits (at most 8)
+// merge as a cluster or there is one; nothing is kept between calls.
+MI_EXPORT int mi_attn_decode_mma_careful(const void* q, int q_stride, const void* k_cache, const void* v_cache, void* out, const int* decode_segs, int num_decode,
+                                         const int* seg_q_start, const int* seg_kv_len, const int* block_table, const int* table_rows, int table_stride, int H,
+                                         int KV, int D, int ps, int splits, float scale, int* error_word, int cache_pages, cudaStream_t stream) {
+    if (splits < 1 || error_word == nullptr || (uintptr_t)q % 16 || num_decode > 0x7fffffff / 8 || KV > 65535) return -2;
+    return decode_mma_rows_launch<false>(q, q_stride, k_cache, v_cache, out, nullptr, nullptr, decode_segs, num_decode, seg_q_start, seg_kv_len, block_table, table_rows,
+                                         table_stride, H, KV, D, ps, splits > 8 ? 8 : splits, scale, 0, nullptr, error_word, cache_pages, 1, stream, 0, 0, nullptr, nullptr, 0,
+                                         nullptr, DecodeExt{0.f, 0, nullptr, 0, 1});
 }
 
 // The same with every softmax weight split into two bfloat16 numbers for the P V product (see SPLIT above).
@@ -705,7 +730,7 @@ MI_EXPORT int mi_attn_decode_mma_rows_capped(const void* q, int q_stride, const 
                                              float scale, int window, int* merge_counters, int* error_word, int cache_pages,
                                              int cluster_merge, float cap, int keep, const void* gate, int gate_stride, cudaStream_t stream) {
     if (gate && splits > 1 && !merge_counters) return -2;
-    const DecodeExt ext{cap, keep, (const __nv_bfloat16*)gate, gate_stride};
+    const DecodeExt ext{cap, keep, (const __nv_bfloat16*)gate, gate_stride, 0};
     return decode_mma_rows_launch<true, false, true>(DECODE_ROWS_ARGS, 0, 0, nullptr, nullptr, 0, nullptr, ext);
 }
 #undef DECODE_ROWS_ARGS

@@ -667,7 +667,7 @@ class CudaOps:
         same, and are read by the pages of the first row that has them all; max_shared_rows, on the host: rows of the largest group (rows beyond it are computed alone).  An entry
         without keys gets zeros.  The output [T, H D] has the entries' rows; others are left as they come.
         Heads of 64 or 128 run on kernels that share; other heads, more than 4,096 entries and groups, bfloat16 pages that neither divide 64 keys nor are divided
-        by them, bfloat16 rows that do not lie whole heads apart, and float32 caches that are small (SHARED_BYTES) are computed row by row, by the rows' own pages."""
+        by them, bfloat16 rows that do not lie whole heads apart, and calls that read little (SHARED_BYTES) are computed row by row, by the rows' own pages."""
         rows = getattr(meta, "table_rows", None)
         lists = (meta.decode_segs, meta.seg_q_start, meta.seg_kv_len, meta.shared_start, meta.shared_len)
         tables = (meta.block_table,) if rows is None else (meta.block_table, rows)
@@ -709,13 +709,31 @@ class CudaOps:
         if self._elsewhere():
             with torch.cuda.device(self._device_index):
                 return self._shared_or_alone(q, k_cache, v_cache, meta, H, KV, D, scale)
-        out = torch.empty_like(q, memory_format=torch.contiguous_format)
-        size = self._shared_bytes(q, k_cache, v_cache, meta, H, KV, D) if q.dtype is torch.bfloat16 or self._sharing_pays(q, meta, KV, D, False) else 0
+        out, bf16 = torch.empty_like(q, memory_format=torch.contiguous_format), q.dtype is torch.bfloat16
+        pays = self._sharing_pays(q, meta, KV, D, bf16)
+        if bf16 and not pays and self._decode_few(q, k_cache, v_cache, out, meta, H, KV, D, scale):
+            return out
+        size = self._shared_bytes(q, k_cache, v_cache, meta, H, KV, D) if bf16 or pays else 0
         if size > 0:
             self._shared_decode(q, k_cache, v_cache, out, meta, H, KV, D, scale, size)
         else:
             self._decode_alone(q, k_cache, v_cache, out, meta, H, KV, D, scale)
         return out
+
+    def _decode_few(self, q, k_cache, v_cache, out, meta, H, KV, D, scale):
+        """Entries one by one on the tensor cores, where that kernel takes them."""
+        if (not self.fast_attention or D not in (64, 128) or H // KV > 16 or meta.page_size % 16 or q.stride(0) % 8
+                or (q.data_ptr() | k_cache.data_ptr() | v_cache.data_ptr()) % 16):
+            return False
+        segs = meta.decode_segs
+        n = len(segs)
+        S = min(8, self.choose_splits(n * KV, meta.max_kv_len, 2, cluster=True, head_dim=D))
+        while S > 1 and not self._cluster_fits(D, S, n * KV):       # the splits merge as clusters, or there are none
+            S -= 1
+        _check(self.lib.mi_attn_decode_mma_careful(q, q.stride(0), k_cache, v_cache, out, segs, n, meta.seg_q_start, meta.seg_kv_len, meta.block_table, getattr(meta, "table_rows", None),
+                                                   meta.max_pages, H, KV, D, meta.page_size, S, scale, self._stream_error, len(k_cache), self._stream()), "attn_decode_mma")
+        self.launches += 1
+        return True
 
     def _decode_alone(self, q, k_cache, v_cache, out, meta, H, KV, D, scale):
         """Entries one by one, each by its own pages, on the kernels that read nothing behind an entry's keys and keep nothing between calls."""
@@ -730,11 +748,11 @@ class CudaOps:
                                                getattr(meta, "table_rows", None), meta.max_pages, H, KV, D, meta.page_size, S, scale, 0, _code(q.dtype), self._stream()), "attn_decode")
         self.launches += 2 if S > 1 else 1
 
-    # What the rows would read one by one, from which on sharing is the faster way: less stays in the L2 cache from one row to the next.  Microseconds, sharing / one by one, 32
-    # heads over 8 of 128.  bfloat16 (paged_attention's decode kernel): 4 rows x 512 keys 15 / 8, 8 x 4,096 (135 MB) 25 / 24, 16 x 2,048 (136 MB) 19 / 24, 4 groups of
-    # 8 x 1,024 (138 MB) 24 / 22, 8 x 8 x 1,024 (277 MB) 30 / 44, 8 x 8 x 4,096 46 / 146.  float32, whose multiply-adds bound the shared form: 13 rows x 1,600 (171 MB) 37 / 31,
-    # 8 x 4,096 (270 MB) 44 / 44, 8 x 8 x 512 (285 MB) 75 / 49, 16 x 4,096 (541 MB) 68 / 78, 8 x 16 x 512 (570 MB) 126 / 97, 8 x 8 x 2,048 (1.1 GB) 137 / 175.
-    # (shared_prefix_attention itself shares bfloat16 at every size: that decode kernel wants finite numbers in the unused ends of pages, a key per entry, and its counters to itself.)
+    # What the rows would read one by one, from which on sharing is the faster way: less stays in the L2 cache from one row to the next, and one launch does for it.
+    # Microseconds, sharing / one by one, 32 heads over 8 of 128.  bfloat16: 4 rows x 512 keys 15 / 8, 16 x 1,024 (69 MB) 18 / 17, 8 x 2,048 (68 MB) 22 / 17, 8 x 4,096
+    # (135 MB) 25 / 26, 16 x 2,048 (136 MB) 19 / 26, 8 groups of 4 x 1,024 (138 MB) 24 / 25, 8 x 8 x 1,024 (277 MB) 30 / 47, 8 x 8 x 4,096 46 / 157.  float32, whose
+    # multiply-adds bound the shared form: 13 rows x 1,600 (171 MB) 37 / 31, 8 x 4,096 (270 MB) 44 / 44, 8 x 8 x 512 (285 MB) 75 / 49, 16 x 4,096 (541 MB) 68 / 78, 8 x
+    # 16 x 512 (570 MB) 126 / 97, 8 x 8 x 2,048 (1.1 GB) 137 / 175.
     SHARED_BYTES = {torch.bfloat16: 128 << 20, torch.float32: 512 << 20}
 
     def _sharing_pays(self, q, meta, KV, D, bf16):

@@ -78,9 +78,10 @@ def problem(groups, H, KV, D, ps, dtype, seed=0, alone=(), garbage=math.nan, ext
 
 @pytest.fixture(params=["by the rule", "shared at any size"], autouse=True)
 def form(request, monkeypatch):
-    """Small float32 caches go to the kernel without sharing; every test runs on both."""
+    """Calls that read little go to the kernels without sharing; every test runs on both."""
     if request.param != "by the rule":
         monkeypatch.setattr(CudaOps, "SHARED_BYTES", {BF16: 0, F32: 0})
+    return request.param
 
 
 def check(ops, q, k, v, meta, H, KV, D, scale=None, got=None):
@@ -120,10 +121,10 @@ SHAPES = [(32, 8, 128, 16, BF16), (40, 8, 128, 16, BF16), (6, 2, 64, 32, BF16), 
 @gpu
 @pytest.mark.parametrize("H,KV,D,ps,dtype", SHAPES)
 @pytest.mark.parametrize("name", GROUPS)
-def test_shared_prefix_attention(ops, name, H, KV, D, ps, dtype):
+def test_shared_prefix_attention(ops, name, H, KV, D, ps, dtype, form):
     q, k, v, meta = problem(GROUPS[name], H, KV, D, ps, dtype, seed=len(name) + D)
-    if (name == "no keys" and ops._shared_bytes(q, k, v, meta, H, KV, D) <= 0):
-        pytest.skip("entries without keys: the kernels that share")
+    if (name == "no keys" and (ops._shared_bytes(q, k, v, meta, H, KV, D) <= 0 or form == "by the rule")):
+        pytest.skip("the first row has no pages, so the others' own may hold other keys than the group's: the kernels that share")
     check(ops, q, k, v, meta, H, KV, D)
 
 
@@ -246,13 +247,22 @@ def test_as_many_entries_as_it_takes(ops):
 
 
 @gpu
-@pytest.mark.parametrize("H,KV,D,ps,dtype", [(6, 3, 48, 4, BF16), (6, 3, 32, 4, F32), (10, 2, 128, 32, F32), (8, 2, 64, 16, F32)])
+@pytest.mark.parametrize("H,KV,D,ps,dtype", [(6, 3, 48, 4, BF16), (6, 3, 32, 4, F32), (10, 2, 128, 32, F32), (8, 2, 64, 16, F32), (32, 8, 128, 16, BF16), (6, 2, 64, 32, BF16)])
 def test_entries_without_keys_computed_alone(ops, H, KV, D, ps, dtype, monkeypatch):
     """Zeros, in one piece and where the longest entry makes several, and nothing of what lies behind the keys."""
-    monkeypatch.setattr(CudaOps, "SHARED_BYTES", {BF16: 0, F32: 1 << 60})
+    monkeypatch.setattr(CudaOps, "SHARED_BYTES", {BF16: 1 << 60, F32: 1 << 60})
     for groups in (GROUPS["no keys"], [(0, [0, 3000, 1]), (700, [700, 0, 701])]):
         q, k, v, meta = problem(groups, H, KV, D, ps, dtype, seed=13)
         check(ops, q, k, v, meta, H, KV, D)
+
+
+@gpu
+@pytest.mark.parametrize("H,KV,D,ps", [(16, 8, 128, 16), (8, 2, 64, 32)])
+@pytest.mark.parametrize("lens", [[255, 257], [2048, 2047, 1], [4097, 4100], [8200], [300, 0, 8100], [1025] * 5, [513] * 17, [700] * 40])
+def test_few_rows_of_all_lengths(ops, lens, H, KV, D, ps):
+    """From one split to eight, blocks of either size, as clusters and without."""
+    q, k, v, meta = problem([(min([n for n in lens if n]) // ps * ps, lens)], H, KV, D, ps, BF16, seed=len(lens))
+    check(ops, q, k, v, meta, H, KV, D)
 
 
 @gpu
