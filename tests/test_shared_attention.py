@@ -239,7 +239,7 @@ def test_pages_beyond_32_bits(ops, dtype):
 @gpu
 def test_as_many_entries_as_it_takes(ops):
     """1,900 rows in groups of four, and more than the kernel takes (computed row by row)."""
-    for n in (475, 900):                                          # (without garbage where rows are computed alone: that kernel multiplies it by zero)
+    for n in (475, 900):                                          # (zeros behind the keys where rows are computed alone; test_what_no_row_sees_stays_out has the other numbers)
         takes = 5 * n <= 4096
         q, k, v, meta = problem([(16, [17, 18, 19, 20])] * n, 4, 1, 64, 16, BF16, seed=12, garbage=math.nan if takes else 0.0)
         assert (ops._shared_bytes(q, k, v, meta, 4, 1, 64) > 0) == takes
