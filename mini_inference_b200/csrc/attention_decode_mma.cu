@@ -392,18 +392,18 @@ attn_decode_mma_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_co
             num += f * smem[((size_t)w * 16 + row) * D + d];
             den += f * sl[w * 16 + row];
         }
-        const float val = den > 0.f ? num / den : 0.f;
+        const float val = den == 0.f ? 0.f : num / den;        // 0: no key; a NaN among the scores is in the sum, and stays
         const int h = kvh * G + row;
         if (S == 1) {
             out[((size_t)tok * H + h) * D + d] = __float2bfloat16_rn(gated(val, h, d));
         } else if (BULK && cluster_merge) {
             float* cpart = smem + CLUSTER_OFF;             // [16][D] this split's rows, then [16] their log-sum-exp
             cpart[idx] = val;
-            if (d == 0) cpart[16 * D + row] = den > 0.f ? (mx + log2f(den)) * 0.6931471805599453f : -INFINITY;
+            if (d == 0) cpart[16 * D + row] = den == 0.f ? -INFINITY : (mx + log2f(den)) * 0.6931471805599453f;
         } else {
             const size_t pi = ((size_t)blockIdx.x * H + h) * S + s;
             o_part[pi * D + d] = val;
-            if (d == 0) lse_part[pi] = den > 0.f ? (mx + log2f(den)) * 0.6931471805599453f : -INFINITY;
+            if (d == 0) lse_part[pi] = den == 0.f ? -INFINITY : (mx + log2f(den)) * 0.6931471805599453f;
         }
     }
     if (BULK && cluster_merge && S > 1) {

@@ -134,7 +134,7 @@ __global__ void attn_decode_split_kernel(const T* __restrict__ q, int q_stride, 
     if (lo < hi)
         attend_range<T>(q_s[warp], k_cache, v_cache, block_table + (size_t)(table_rows ? table_rows[seg] : seg) * table_stride, kvh, KV, D, ps,
                         lo, hi, m, l, acc);
-    const float inv = l > 0.f ? 1.f / l : 0.f;                  // empty piece: output 0, lse -inf
+    const float inv = l == 0.f ? 0.f : 1.f / l;                 // empty piece: output 0, lse -inf; a NaN among the scores is in the sum, and stays
     if (S == 1) {
         T* orow = out + ((size_t)tok * H + h) * D;
 #pragma unroll
@@ -144,7 +144,7 @@ __global__ void attn_decode_split_kernel(const T* __restrict__ q, int q_stride, 
         float* orow = o_part + idx * D;
 #pragma unroll
         for (int k = 0; k < MAX_D / 32; ++k) { const int d = lane + 32 * k; if (d < D) orow[d] = acc[k] * inv; }
-        if (lane == 0) lse_part[idx] = l > 0.f ? m + logf(l) : -INFINITY;
+        if (lane == 0) lse_part[idx] = l == 0.f ? -INFINITY : m + logf(l);
     }
 }
 
