@@ -240,7 +240,7 @@ __global__ void __launch_bounds__(128 * PARTS, PARTS == 2 ? 4 : 1) merge_kernel(
                 float sum = 0.f;
                 for (int i = lane; i < now; i += 32) {
                     const float2 ml = i < 32 ? first : piece(i);
-                    const float w = exp2f(ml.x - off);
+                    const float w = isnan(ml.y) ? ml.y : exp2f(ml.x - off);      // maxima pass NaN scores over, sums do not: the row is NaN
                     weight[i * HEADS + warp] = w;
                     if (w != 0.f) sum = fmaf(ml.y, w, sum);
                 }

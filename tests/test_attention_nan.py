@@ -5,6 +5,7 @@ import math
 import pytest
 import torch
 
+from mini_inference_b200.ops import CudaOps
 from tests.ref_beam import shared_prefix_attention64
 from tests.test_shared_attention import BF16, F32, problem
 
@@ -91,3 +92,18 @@ def test_small_calls_of_the_operator(ops, H, KV, D, ps, dtype, where):
         got = ops.shared_prefix_attention(q, k, v, meta, H, KV, D, 0.1)
         ops.check_errors()
         check_nan(q, k, v, meta, H, KV, D, 0.1, got)
+
+
+@gpu
+@pytest.mark.parametrize("where", WHERE)
+@pytest.mark.parametrize("H,KV,D,ps,dtype", [(8, 2, 128, 16, BF16), (32, 8, 128, 16, BF16), (6, 2, 64, 32, BF16), (16, 1, 128, 64, BF16), (6, 2, 64, 16, F32), (8, 2, 128, 16, F32)])
+def test_shared_prefixes(ops, monkeypatch, H, KV, D, ps, dtype, where):
+    """On the kernels that share: prefixes and tails of one piece and of many, tails of a single key, rows alone."""
+    monkeypatch.setattr(CudaOps, "SHARED_BYTES", {BF16: 0, F32: 0})
+    for groups in ([(64, [65, 65, 90])], [(0, [1, 1, 3])], [(2048, [2049, 2500, 2060, 2048]), (128, [129, 140])], [(512, [513] * 33), (64, [0, 70, 65])], [(4096, [4200, 6000])]):
+        q, k, v, meta = spoiled(groups, H, KV, D, ps, dtype, where, seed=D, alone=(1, 300))
+        assert ops._shared_bytes(q, k, v, meta, H, KV, D) > 0
+        got = ops.shared_prefix_attention(q, k, v, meta, H, KV, D, 0.1)
+        ops.check_errors()
+        want = check_nan(q, k, v, meta, H, KV, D, 0.1, got)
+        assert want.isnan().any()
