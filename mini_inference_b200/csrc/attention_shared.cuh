@@ -1,7 +1,9 @@
 // Decode attention over a shared prefix: the work that attention_shared_tc.cu (bfloat16, tensor cores) and attention_shared_f32.cu share.
 //
 // Rows (one fed token each) come in groups; group g's rows all begin with the same shared_len[g] keys, which are read by the pages of the first row that holds
-// them all, once for all rows and query heads of the group, and every row has a tail of its own.  The softmax over both is joined from running maxima and sums:
+// them all, once for all rows and query heads of the group that hold them all, and every row has a tail of its own.  A row that ends in front of shared_len[g] has
+// all its keys in its tail: in a prefix's tile its weights behind its end would be 0, and 0 times an infinite value that another row sees is no 0.  Where every
+// row ends there the group has no prefix part.  The softmax over both is joined from running maxima and sums:
 //     o = sum_i e^(m_i - M) o_i / sum_i e^(m_i - M) l_i   over the pieces i that a row's keys were cut into, M = max_i m_i.
 //
 // Items of work, in this order: (group, key head, tile of the group's rows) over the prefix, then (row, key head) over the tail, each a number of tiles of KT
@@ -41,8 +43,8 @@ struct __align__(16) Record {                        // where a row's pieces are
 // Copy s of row i is row s rows + i of the piece's place.
 __host__ __device__ __forceinline__ int copies_of(int copies, int rows) { return !copies || rows > 64 ? 1 : rows > 32 ? 2 : 4; }
 
-// in shared memory: sums of tiles [G + R + 1]; a row's first tail key, group (-1: none), keys, token and row of the block table [R] each; a group's first row, rows,
-// shared keys and the row whose pages hold them [G] each
+// in shared memory: sums of tiles [G + R + 1]; a row's first tail key (0: it takes no part in a prefix), group (-1: none), keys, token and row of the block table [R]
+// each; a group's first row, rows, shared keys and the row whose pages hold them [G] each
 struct Plan {
     int *sums, *first, *group, *keys, *token, *table, *start, *rows, *shared, *source;
     __device__ __forceinline__ Plan(int* mem, int G, int R)
@@ -65,7 +67,6 @@ __device__ __forceinline__ void make_plan(const Args& a, const Plan& p) {
         const int start = max(0, min(a.shared_start[g], a.R)), n = min(max(0, min(a.shared_start[g + 1], a.R) - start), a.most);
         const int keys = n > 1 ? max(0, min(a.shared_len[g], a.table_stride * a.ps)) : 0;
         p.start[g] = start; p.rows[g] = n; p.shared[g] = keys; p.source[g] = start + n;
-        p.sums[g + 1] = a.KV * ((n + a.tile_rows - 1) / a.tile_rows) * with_pad((keys + KT - 1) / KT);
     }
     for (int r = threadIdx.x; r < a.R; r += blockDim.x) {
         // entry r is most often entry decode_segs[r]: its numbers are asked for beside it, not behind it
@@ -81,11 +82,17 @@ __device__ __forceinline__ void make_plan(const Args& a, const Plan& p) {
         int g = 0, right = a.G;                      // the last group that starts at or in front of row r
         while (right - g > 1) { const int mid = (g + right) / 2; if (p.start[mid] <= r) g = mid; else right = mid; }
         const bool in = a.G > 0 && r >= p.start[g] && r < p.start[g] + p.rows[g];
-        const int len = p.keys[r], first = in ? p.shared[g] : 0;
+        const int len = p.keys[r], shared = in ? p.shared[g] : 0, first = len >= shared ? shared : 0;
         p.group[r] = in ? g : -1;
         p.first[r] = first;
-        if (first > 0 && len >= first) atomicMin(&p.source[g], r);
+        if (first > 0) atomicMin(&p.source[g], r);
         p.sums[a.G + r + 1] = len > first ? a.KV * with_pad((len - tail_base(a, first, KT) + KT - 1) / KT) : 0;
+    }
+    __syncthreads();
+    for (int g = threadIdx.x; g < a.G; g += blockDim.x) {
+        const int n = p.rows[g];
+        if (p.source[g] == p.start[g] + n) p.shared[g] = 0;      // nobody has them all
+        p.sums[g + 1] = a.KV * ((n + a.tile_rows - 1) / a.tile_rows) * with_pad((p.shared[g] + KT - 1) / KT);
     }
     if (threadIdx.x == 0) p.sums[0] = 0;
     __syncthreads();
@@ -106,7 +113,7 @@ __device__ __forceinline__ void make_plan(const Args& a, const Plan& p) {
         for (int r = threadIdx.x; r < a.R; r += blockDim.x) {
             const int g = p.group[r], at = p.sums[a.G + r];
             Record rec{p.token[r], 0, 0, 0, 0, 0, at, (p.sums[a.G + r + 1] - at) / a.KV};
-            if (g >= 0) {
+            if (p.first[r] > 0) {
                 const int start = p.start[g], tm = (p.rows[g] + a.tile_rows - 1) / a.tile_rows, mt = (r - start) / a.tile_rows;
                 rec.prefix_tiles = with_pad((p.shared[g] + KT - 1) / KT);
                 rec.prefix_at = p.sums[g] + mt * rec.prefix_tiles;
@@ -166,11 +173,9 @@ struct Walk {
             if (tiles > 0) return true;
         }
     }
-    __device__ __forceinline__ int table_row() const {
-        int holds = who;
-        if (prefix) { holds = p.source[who]; if (holds >= p.start[who] + p.rows[who]) holds = p.start[who]; }      // nobody has them all
-        return p.table[holds];
-    }
+    __device__ __forceinline__ int table_row() const { return p.table[prefix ? p.source[who] : who]; }
+    // row r of the piece sees its keys below this: a row that is no part of a prefix none
+    __device__ __forceinline__ int end_of(int r) const { return prefix ? min(hi, p.first[row0 + r]) : hi; }
     __device__ __forceinline__ int place() const { return (prefix ? (who * a.KV + kvh) * a.row_tiles + row_tile : who * a.KV + kvh) + (int)blockIdx.x; }
 };
 

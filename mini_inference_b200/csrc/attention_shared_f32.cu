@@ -71,7 +71,7 @@ __global__ void __launch_bounds__(THREADS, 2) attn_shared_f32_kernel(const __gri
                 *reinterpret_cast<const float4*>(q + (size_t)plan.token[r] * q_stride + (size_t)h * D + c);
         }
         const int my_row = tid >> 3;                 // softmax: eight threads a row
-        const int hi = my_row < rows ? min(walk.hi, plan.keys[walk.row0 + my_row / Hg]) : 0;
+        const int hi = my_row < rows ? walk.end_of(my_row / Hg) : 0;
         float m = -INFINITY, l = 0.f, acc[4][C];
 #pragma unroll
         for (int i = 0; i < 4; ++i)

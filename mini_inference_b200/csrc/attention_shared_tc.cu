@@ -315,8 +315,8 @@ attn_shared_tc_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_con
             const int copies = copies_of(1, rows), warps = 4 / copies, copy = lg / warps, col = copy * (KT / copies);
             const int mine = lg % warps * 32 + lane - (rows <= 16 && piece & 1 ? 16 : 0);      // the row
             const bool there = mine >= 0 && mine < rows, active = __any_sync(0xffffffffu, there);
-            // a prefix's rows see no further than their own length; lanes beyond the rows hold anything
-            const int mine_hi = there ? min(hi, plan.keys[at.row0 + mine / Hg]) : hi;
+            // as Walk::end_of; lanes beyond the rows hold anything
+            const int mine_hi = there && at.prefix ? min(hi, plan.first[at.row0 + mine / Hg]) : hi;
             Row row{-INFINITY, 0.f};
             for (int i = 0; i < tiles && ok; ++i, ++n) {
                 const int s = n & 1, key = at.key0 + i * KT;

@@ -664,8 +664,9 @@ class CudaOps:
         q [T, H D] (rows may be strided), caches [pages, KV, page_size, D].  meta: decode_segs int32 [R] (the entries, one fed token each), seg_q_start, seg_kv_len,
         block_table and table_rows as paged_attention reads them (max_kv_len: the longest); shared_start int32 [G + 1]: entries decode_segs[shared_start[g]] ..
         decode_segs[shared_start[g + 1] - 1] are group g (rows in no group stand alone), shared_len int32 [G]: the first so many keys of its rows are the
-        same, and are read by the pages of the first row that has them all; max_shared_rows, on the host: rows of the largest group (rows beyond it are computed alone).  An entry
-        without keys gets zeros.  The output [T, H D] has the entries' rows; others are left as they come.
+        same, and are read by the pages of the first row that has them all (a row that has fewer is computed by its own pages); max_shared_rows, on the host: rows of the largest
+        group (rows beyond it are computed alone).  An entry without keys gets zeros.  The output [T, H D] has the entries' rows; others are left as they come.  What lies behind
+        an entry's keys counts for nothing; NaN among the keys and queries that it sees makes it NaN, and a value that is not finite makes its column not finite.
         Heads of 64 or 128 run on kernels that share; other heads, more than 4,096 entries and groups, bfloat16 pages that neither divide 64 keys nor are divided
         by them, bfloat16 rows that do not lie whole heads apart, and calls that read little (SHARED_BYTES) are computed row by row, by the rows' own pages."""
         rows = getattr(meta, "table_rows", None)
