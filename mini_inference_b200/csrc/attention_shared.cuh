@@ -10,8 +10,9 @@
 // keys.  All tiles of all items stand in one line, PAD empty ones in front of each item's (what beginning and ending an item costs), and block c of a grid that
 // fills the GPU once takes tiles [c per, (c + 1) per): every block has the same work whatever the lengths are, long prefixes are cut over many blocks
 // and short tails put together in one.  A block's share of one item is a
-// piece; it is kept at place item + c (items and blocks both grow along the line, so no two pieces share a place).  How many tiles each group and row has
-// is known on the device alone; every block adds them up for itself (a few hundred numbers), block 0 leaves the sums for the merge.
+// piece.  Its rows are kept from row at(item) + c places of the largest piece on, where at leaves each item the room of its own rows: items and blocks both grow
+// along the line, so no two pieces share a row, and all prefixes together take what their groups' rows take, however unlike the groups are.  How many tiles each
+// group and row has is known on the device alone; every block adds them up for itself (a few hundred numbers), block 0 leaves the sums for the merge.
 // A group of one row has no prefix part: its whole length is its tail.
 #pragma once
 #include "common.cuh"
@@ -26,22 +27,24 @@ constexpr int MAX_ENTITIES = 4096;                   // groups + rows of a call
 struct Args {
     const int *decode_segs, *seg_q_start, *seg_kv_len, *block_table, *table_rows, *shared_start, *shared_len;
     int R, G, entries, most, table_stride, H, KV, ps;  // most: rows of the largest group; rows beyond it have no prefix part
-    int row_tiles, tile_rows;                        // tiles of rows of the largest group; rows of a tile (x H / KV heads = its matrix rows)
+    int tile_rows;                                   // rows of a tile (x H / KV heads = its matrix rows)
     int copies;                                      // 1: a piece's keys may be shared out over up to 4 copies of its rows (see copies_of)
-    int slot_rows, tail_rows;                        // rows of a prefix piece's place and of a tail piece's, copies among them
-    float *o_prefix, *o_tail;                        // [places][D / 4][rows of a place][4], not divided by the sums: neighbouring rows' 16 bytes side by side
-    float2 *ml_prefix, *ml_tail;                     // [places][rows of a place]: maximum (base 2) and sum
+    int slot_rows, tail_rows;                        // matrix rows of the largest prefix piece and of a tail's, copies among them
+    float *o_prefix, *o_tail;                        // [rows] D numbers, a piece's as [D / 4][its rows][4]: not divided by the sums, neighbouring rows' 16 bytes side by side
+    float2 *ml_prefix, *ml_tail;                     // [rows]: maximum (base 2) and sum
     int* plan;                                       // what block 0 leaves for the merge: tiles of a block, and a Record per row
 };
 
 struct __align__(16) Record {                        // where a row's pieces are: its token; the prefix item of key head 0 (first tile, tiles to the next key head's,
-    int token, prefix_at, prefix_step, prefix_tiles; // tiles, place, first matrix row) and the tail's (first tile, tiles)
-    int prefix_place, prefix_row, tail_at, tail_tiles;      // prefix_row: the tile's rows in the upper half
+    int token, prefix_at, prefix_step, prefix_tiles; // tiles, where its pieces' rows begin, rows to the next key head's, first matrix row) and the tail's (first tile, tiles)
+    int prefix_place, prefix_head, prefix_row, tail_at, tail_tiles;      // prefix_row: the tile's rows in the upper half
 };
 
 // How often a piece of so many rows has each of them: the copies' keys are different columns of a tile, so each is a piece of its own to the merge.
-// Copy s of row i is row s rows + i of the piece's place.
+// Copy s of row i is row s rows + i of the piece.
 __host__ __device__ __forceinline__ int copies_of(int copies, int rows) { return !copies || rows > 64 ? 1 : rows > 32 ? 2 : 4; }
+// Rows that a batch row's heads may take in a prefix piece: group g's items have this many from row room start[g] KV on (groups do not overlap)
+__host__ __device__ __forceinline__ int room_of(int copies, int H, int KV) { return (copies ? 4 : 1) * (H / KV); }
 
 // in shared memory: sums of tiles [G + R + 1]; a row's first tail key (0: it takes no part in a prefix), group (-1: none), keys, token and row of the block table [R]
 // each; a group's first row, rows, shared keys and the row whose pages hold them [G] each
@@ -58,6 +61,11 @@ __device__ __forceinline__ int tail_base(const Args& a, int first, int KT) { con
 // tiles of an item in the line
 __device__ __forceinline__ int with_pad(int tiles) { return tiles > 0 ? tiles + PAD : 0; }
 __device__ __forceinline__ int tiles_of_a_block(int total) { return max(1, (total + (int)gridDim.x - 1) / (int)gridDim.x); }
+
+// where the rows of a group's pieces begin, by key head and tile of rows
+__device__ __forceinline__ int prefix_at(const Args& a, const Plan& p, int g, int kvh, int row_tile) {
+    return room_of(a.copies, a.H, a.KV) * (p.start[g] * a.KV + kvh * p.rows[g] + row_tile * a.tile_rows);
+}
 
 // Called by all threads of a block; afterwards (and a barrier) the sums stand in shared memory.
 template <int KT>
@@ -112,13 +120,14 @@ __device__ __forceinline__ void make_plan(const Args& a, const Plan& p) {
         Record* records = reinterpret_cast<Record*>(a.plan + 4);
         for (int r = threadIdx.x; r < a.R; r += blockDim.x) {
             const int g = p.group[r], at = p.sums[a.G + r];
-            Record rec{p.token[r], 0, 0, 0, 0, 0, at, (p.sums[a.G + r + 1] - at) / a.KV};
+            Record rec{p.token[r], 0, 0, 0, 0, 0, 0, at, (p.sums[a.G + r + 1] - at) / a.KV};
             if (p.first[r] > 0) {
                 const int start = p.start[g], tm = (p.rows[g] + a.tile_rows - 1) / a.tile_rows, mt = (r - start) / a.tile_rows;
                 rec.prefix_tiles = with_pad((p.shared[g] + KT - 1) / KT);
                 rec.prefix_at = p.sums[g] + mt * rec.prefix_tiles;
                 rec.prefix_step = tm * rec.prefix_tiles;
-                rec.prefix_place = g * a.KV * a.row_tiles + mt;
+                rec.prefix_place = prefix_at(a, p, g, 0, mt);
+                rec.prefix_head = room_of(a.copies, a.H, a.KV) * p.rows[g];
                 rec.prefix_row = (r - start) % a.tile_rows * (a.H / a.KV) | min(a.tile_rows, p.rows[g] - mt * a.tile_rows) * (a.H / a.KV) << 16;
             }
             records[r] = rec;
@@ -176,7 +185,9 @@ struct Walk {
     __device__ __forceinline__ int table_row() const { return p.table[prefix ? p.source[who] : who]; }
     // row r of the piece sees its keys below this: a row that is no part of a prefix none
     __device__ __forceinline__ int end_of(int r) const { return prefix ? min(hi, p.first[row0 + r]) : hi; }
-    __device__ __forceinline__ int place() const { return (prefix ? (who * a.KV + kvh) * a.row_tiles + row_tile : who * a.KV + kvh) + (int)blockIdx.x; }
+    __device__ __forceinline__ int place() const {   // the piece's first row
+        return prefix ? prefix_at(a, p, who, kvh, row_tile) + (int)blockIdx.x * a.slot_rows : (who * a.KV + kvh + (int)blockIdx.x) * a.tail_rows;
+    }
 };
 
 // A piece as one warp of a block writes it down for the others (finding it costs a thousand clocks)
@@ -196,7 +207,7 @@ __global__ void __launch_bounds__(128 * PARTS, PARTS == 2 ? 4 : 1) merge_kernel(
     const int r = blockIdx.x, kvh = blockIdx.y, Hg = a.H / a.KV, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int per = a.plan[0];
     const Record rec = reinterpret_cast<const Record*>(a.plan + 4)[r];
-    // pieces of the prefix, then of the tail, every copy of the row one of them; a part's places follow on one another
+    // pieces of the prefix, then of the tail, every copy of the row one of them; a part's pieces lie slot_rows or tail_rows apart
     const int rows_p = rec.prefix_row >> 16, copies_p = copies_of(a.copies, rows_p), copies_t = copies_of(a.copies, Hg);
     const int shift_p = copies_p >> 1, shift_t = copies_t >> 1;        // log2 of 1, 2, 4
     int n_p = 0, n_t = 0;
@@ -204,12 +215,12 @@ __global__ void __launch_bounds__(128 * PARTS, PARTS == 2 ? 4 : 1) merge_kernel(
     if (rec.prefix_tiles > 0) {
         const int t0 = rec.prefix_at + kvh * rec.prefix_step;
         n_p = ((t0 + rec.prefix_tiles - 1) / per - (t0 + PAD) / per + 1) << shift_p;
-        at_p = (size_t)rec.prefix_place + (size_t)kvh * a.row_tiles + (t0 + PAD) / per;
+        at_p = (size_t)rec.prefix_place + (size_t)kvh * rec.prefix_head + (size_t)((t0 + PAD) / per) * a.slot_rows;
     }
     if (rec.tail_tiles > 0) {
         const int t0 = rec.tail_at + kvh * rec.tail_tiles;
         n_t = ((t0 + rec.tail_tiles - 1) / per - (t0 + PAD) / per + 1) << shift_t;
-        at_t = (size_t)r * a.KV + kvh + (t0 + PAD) / per;
+        at_t = ((size_t)r * a.KV + kvh + (t0 + PAD) / per) * a.tail_rows;
     }
     const int n = n_p + n_t;
     for (int h0 = 0; h0 < Hg; h0 += HEADS) {
@@ -219,9 +230,9 @@ __global__ void __launch_bounds__(128 * PARTS, PARTS == 2 ? 4 : 1) merge_kernel(
         float m = -INFINITY, l = 0.f;                // of this warp's head
         float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
         const auto rows_of = [&](int i) {            // this thread's columns of piece i
-            if (i < n_p) return reinterpret_cast<const float4*>(a.o_prefix) + ((at_p + (i >> shift_p)) * (D / 4) + c) * a.slot_rows + (i & (copies_p - 1)) * rows_p + row_p + h;
+            if (i < n_p) return reinterpret_cast<const float4*>(a.o_prefix) + (at_p + (i >> shift_p) * a.slot_rows) * (D / 4) + (c << shift_p) * rows_p + (i & (copies_p - 1)) * rows_p + row_p + h;
             i -= n_p;
-            return reinterpret_cast<const float4*>(a.o_tail) + ((at_t + (i >> shift_t)) * (D / 4) + c) * a.tail_rows + (i & (copies_t - 1)) * Hg + row_t + h;
+            return reinterpret_cast<const float4*>(a.o_tail) + (at_t + (i >> shift_t) * a.tail_rows) * (D / 4) + c * a.tail_rows + (i & (copies_t - 1)) * Hg + row_t + h;
         };
         constexpr int EARLY = 5;                     // pieces of a thread that are asked for before their weights are there
         float4 early[EARLY];
@@ -233,9 +244,9 @@ __global__ void __launch_bounds__(128 * PARTS, PARTS == 2 ? 4 : 1) merge_kernel(
             if (warp < heads) {
                 const auto piece = [&](int i) {
                     i += i0;
-                    if (i < n_p) return a.ml_prefix[(at_p + (i >> shift_p)) * a.slot_rows + (i & (copies_p - 1)) * rows_p + row_p + warp];
+                    if (i < n_p) return a.ml_prefix[at_p + (i >> shift_p) * a.slot_rows + (i & (copies_p - 1)) * rows_p + row_p + warp];
                     i -= n_p;
-                    return a.ml_tail[(at_t + (i >> shift_t)) * a.tail_rows + (i & (copies_t - 1)) * Hg + row_t + warp];
+                    return a.ml_tail[at_t + (i >> shift_t) * a.tail_rows + (i & (copies_t - 1)) * Hg + row_t + warp];
                 };
                 const float2 first = lane < now ? piece(lane) : make_float2(-INFINITY, 0.f);
                 float top = fmaxf(m, first.x);
@@ -304,18 +315,18 @@ template <typename Kernel> inline cudaError_t allow_shared(Kernel kernel, int by
     return e;
 }
 
-// Scratch of a call: floats of o_prefix, o_tail, then float2 of both, then the plan
+// Scratch of a call: floats of o_prefix, o_tail, then float2 of both, then the plan.  bytes -2: rows that do not fit an int
 struct Scratch { long long o_prefix, o_tail, ml_prefix, ml_tail, plan, bytes; };
-inline Scratch scratch(int R, int G, int KV, int D, int row_tiles, int slot_rows, int tail_rows, int blocks) {
-    const long long places_p = (long long)G * KV * row_tiles + blocks, places_t = (long long)R * KV + blocks;
+inline Scratch scratch(const Args& a, int D, int blocks) {
+    const long long rows_p = (long long)room_of(a.copies, a.H, a.KV) * a.R * a.KV + (long long)blocks * a.slot_rows, rows_t = ((long long)a.R * a.KV + blocks) * a.tail_rows;
     const auto up = [](long long v) { return (v + 255) / 256 * 256; };
     Scratch s;
     s.o_prefix = 0;
-    s.o_tail = s.o_prefix + up(places_p * slot_rows * D * 4);
-    s.ml_prefix = s.o_tail + up(places_t * tail_rows * D * 4);
-    s.ml_tail = s.ml_prefix + up(places_p * slot_rows * 8);
-    s.plan = s.ml_tail + up(places_t * tail_rows * 8);
-    s.bytes = s.plan + up(16 + (long long)R * sizeof(Record));
+    s.o_tail = s.o_prefix + up(rows_p * D * 4);
+    s.ml_prefix = s.o_tail + up(rows_t * D * 4);
+    s.ml_tail = s.ml_prefix + up(rows_p * 8);
+    s.plan = s.ml_tail + up(rows_t * 8);
+    s.bytes = rows_p > 0x7fffffff || rows_t > 0x7fffffff ? -2 : s.plan + up(16 + (long long)a.R * sizeof(Record));
     return s;
 }
 inline void place_scratch(Args& a, const Scratch& s, void* work) {

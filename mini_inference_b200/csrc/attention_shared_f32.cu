@@ -149,9 +149,8 @@ __global__ void __launch_bounds__(THREADS, 2) attn_shared_f32_kernel(const __gri
             }
             __syncthreads();                         // the stage, the scores and (behind the last tile) the queries are free
         }
-        const int rows_of = walk.prefix ? a.slot_rows : Hg;
-        const size_t at = (size_t)walk.place() * rows_of;
-        float* o = (walk.prefix ? a.o_prefix : a.o_tail) + at * D + (C * lane / 4 * rows_of + 4 * warp) * 4 + C * lane % 4;
+        const size_t at = (size_t)walk.place();
+        float* o = (walk.prefix ? a.o_prefix : a.o_tail) + at * D + (C * lane / 4 * rows + 4 * warp) * 4 + C * lane % 4;
 #pragma unroll
         for (int r = 0; r < 4; ++r)
             if (4 * warp + r < rows) {
@@ -167,16 +166,21 @@ bool fits(int R, int G, int H, int KV, int D, int ps) {
     return R > 0 && G >= 0 && R + G <= MAX_ENTITIES && KV > 0 && KV <= 65535 && H % KV == 0 && H / KV <= M && (D == 64 || D == 128) && ps > 0;
 }
 int tile_rows_of(int H, int KV) { return M / (H / KV); }
-int row_tiles_of(int H, int KV, int most) { const int t = tile_rows_of(H, KV); return most > 1 ? (most + t - 1) / t : 1; }
 int slot_rows_of(int H, int KV, int most) { const int t = tile_rows_of(H, KV); return (most < t ? (most > 1 ? most : 1) : t) * (H / KV); }
+// a call's sizes, without its pointers
+Args sizes(int R, int G, int entries, int most, int table_stride, int H, int KV, int ps) {
+    Args a = {};
+    a.R = R; a.G = G; a.entries = entries; a.most = most > R ? R : most > 1 ? most : 1; a.table_stride = table_stride; a.H = H; a.KV = KV; a.ps = ps;
+    a.tile_rows = tile_rows_of(H, KV); a.copies = 0; a.slot_rows = slot_rows_of(H, KV, a.most); a.tail_rows = H / KV;
+    return a;
+}
 
 }  // namespace
 
 // Bytes of the work space of a call; -2: sizes that this kernel does not take.  most: rows of the largest group.
 MI_EXPORT long long mi_attn_shared_f32_bytes(int R, int G, int most, int H, int KV, int D, int ps) {
     if (!fits(R, G, H, KV, D, ps)) return -2;
-    most = most > R ? R : most;
-    return scratch(R, G, KV, D, row_tiles_of(H, KV, most), slot_rows_of(H, KV, most), H / KV, 2 * device_sms()).bytes;
+    return scratch(sizes(R, G, 1, most, 0, H, KV, ps), D, 2 * device_sms()).bytes;
 }
 
 // As mi_attn_shared_tc, in float32.
@@ -187,10 +191,12 @@ MI_EXPORT int mi_attn_shared_f32(const float* q, int q_stride, const float* k_ca
     if (R == 0) return 0;
     if (!fits(R, G, H, KV, D, ps) || entries < 1 || q_stride % 4 || (((uintptr_t)q | (uintptr_t)k_cache | (uintptr_t)v_cache | (uintptr_t)work) % 16)) return -2;
     const int blocks = 2 * device_sms();
-    most = most > R ? R : most;
-    Args a{decode_segs, seg_q_start, seg_kv_len, block_table, table_rows, shared_start, shared_len, R, G, entries, most > 1 ? most : 1, table_stride, H, KV, ps,
-           row_tiles_of(H, KV, most), tile_rows_of(H, KV), 0, slot_rows_of(H, KV, most), H / KV};
-    place_scratch(a, scratch(R, G, KV, D, a.row_tiles, a.slot_rows, a.tail_rows, blocks), work);
+    Args a = sizes(R, G, entries, most, table_stride, H, KV, ps);
+    a.decode_segs = decode_segs; a.seg_q_start = seg_q_start; a.seg_kv_len = seg_kv_len; a.block_table = block_table; a.table_rows = table_rows;
+    a.shared_start = shared_start; a.shared_len = shared_len;
+    const Scratch s = scratch(a, D, blocks);
+    if (s.bytes < 0) return -2;
+    place_scratch(a, s, work);
     const float scale_log2 = scale * 1.4426950408889634f;
 #define LAUNCH(DD) do { \
         const size_t smem = (size_t)Tiles<DD>::END * 4, plan = (size_t)plan_ints(G, R) * 4; \

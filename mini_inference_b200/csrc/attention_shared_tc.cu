@@ -364,8 +364,8 @@ attn_shared_tc_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_con
             if (!mbar_wait(pv_done, (n - 1) & 1)) { atomicExch(error_word, 70); break; }
             tc_fence_after();
             if (active) {
-                const int rows_of = at.prefix ? a.slot_rows : a.tail_rows, line = copy * rows + mine;
-                float4* to = reinterpret_cast<float4*>(at.prefix ? a.o_prefix : a.o_tail) + (size_t)at.place * (D / 4) * rows_of + line;
+                const int rows_of = copies * rows, line = copy * rows + mine;
+                float4* to = reinterpret_cast<float4*>(at.prefix ? a.o_prefix : a.o_tail) + (size_t)at.place * (D / 4) + line;
 #pragma unroll 1
                 for (int c = 0; c < D / 32; ++c) {
                     uint32_t o[32];
@@ -377,7 +377,7 @@ attn_shared_tc_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_con
                             to[(size_t)(c * 8 + v4) * rows_of] = make_float4(__uint_as_float(o[4 * v4]), __uint_as_float(o[4 * v4 + 1]), __uint_as_float(o[4 * v4 + 2]), __uint_as_float(o[4 * v4 + 3]));
                     }
                 }
-                if (there) (at.prefix ? a.ml_prefix : a.ml_tail)[(size_t)at.place * rows_of + line] = make_float2(row.m, row.l);
+                if (there) (at.prefix ? a.ml_prefix : a.ml_tail)[(size_t)at.place + line] = make_float2(row.m, row.l);
             }
             tc_fence_before();
             mbar_arrive(o_free);
@@ -419,20 +419,25 @@ bool fits(int R, int G, int H, int KV, int D, int ps) {
            (ps <= KT ? KT % ps == 0 : ps % KT == 0) && KV <= 65535;
 }
 int tile_rows_of(int H, int KV) { return BQ / (H / KV); }
-int row_tiles_of(int H, int KV, int most) { const int t = tile_rows_of(H, KV); return most > 1 ? (most + t - 1) / t : 1; }
 int slot_rows_of(int H, int KV, int most) {          // with the copies of any number of rows up to the largest tile's
     const int t = tile_rows_of(H, KV), rows = (most < t ? (most > 1 ? most : 1) : t) * (H / KV);
     return rows <= BQ / 4 ? 4 * rows : BQ;
 }
 int tail_rows_of(int H, int KV) { return copies_of(1, H / KV) * (H / KV); }
+// a call's sizes, without its pointers
+Args sizes(int R, int G, int entries, int most, int table_stride, int H, int KV, int ps) {
+    Args a = {};
+    a.R = R; a.G = G; a.entries = entries; a.most = most > R ? R : most > 1 ? most : 1; a.table_stride = table_stride; a.H = H; a.KV = KV; a.ps = ps;
+    a.tile_rows = tile_rows_of(H, KV); a.copies = 1; a.slot_rows = slot_rows_of(H, KV, a.most); a.tail_rows = tail_rows_of(H, KV);
+    return a;
+}
 
 }  // namespace
 
 // Bytes of the work space of a call; -2: sizes that this kernel does not take.  most: rows of the largest group.
 MI_EXPORT long long mi_attn_shared_tc_bytes(int R, int G, int most, int H, int KV, int D, int ps) {
     if (!fits(R, G, H, KV, D, ps)) return -2;
-    most = most > R ? R : most;
-    return scratch(R, G, KV, D, row_tiles_of(H, KV, most), slot_rows_of(H, KV, most), tail_rows_of(H, KV), 2 * device_sms()).bytes;
+    return scratch(sizes(R, G, 1, most, 0, H, KV, ps), D, 2 * device_sms()).bytes;
 }
 
 // q, out bfloat16 ([tokens, H D], rows of q q_stride apart); caches [pages, KV, ps, D] with cache_rows = pages KV ps; decode_segs int32 [R] (which of the `entries` feed one token
@@ -447,10 +452,12 @@ MI_EXPORT int mi_attn_shared_tc(const void* q, int q_stride, int tokens, const v
     if (!query_map(q, tokens, H, D, q_stride, H / KV, &qmap)) return -5;
     if (!cache_map(k_cache, cache_rows, D, ps < KT ? ps : KT, &kmap) || !cache_map(v_cache, cache_rows, D, ps < KT ? ps : KT, &vmap)) return -5;
     const int blocks = 2 * device_sms();
-    most = most > R ? R : most;
-    Args a{decode_segs, seg_q_start, seg_kv_len, block_table, table_rows, shared_start, shared_len, R, G, entries, most > 1 ? most : 1, table_stride, H, KV, ps,
-           row_tiles_of(H, KV, most), tile_rows_of(H, KV), 1, slot_rows_of(H, KV, most), tail_rows_of(H, KV)};
-    place_scratch(a, scratch(R, G, KV, D, a.row_tiles, a.slot_rows, a.tail_rows, blocks), work);
+    Args a = sizes(R, G, entries, most, table_stride, H, KV, ps);
+    a.decode_segs = decode_segs; a.seg_q_start = seg_q_start; a.seg_kv_len = seg_kv_len; a.block_table = block_table; a.table_rows = table_rows;
+    a.shared_start = shared_start; a.shared_len = shared_len;
+    const Scratch s = scratch(a, D, blocks);
+    if (s.bytes < 0) return -2;
+    place_scratch(a, s, work);
     const auto bytes = [&](int ints) { return (size_t)BQ * D * 2 + 4 * (size_t)KT * D * 2 + 26 * 8 + PIECES * sizeof(Piece) + (size_t)ints * 4 + 1024; };
     const size_t smem = bytes(plan_ints(G, R)), most_smem = bytes(6 * MAX_ENTITIES + 1);
     const float scale_log2 = scale * LOG2E;

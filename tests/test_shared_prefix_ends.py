@@ -58,3 +58,29 @@ def test_infinite_values_that_only_longer_rows_see(ops, H, KV, D, ps, dtype):   
         sees = torch.zeros(D, dtype=torch.bool)
         sees[[7, 9]] = n > at
         assert near[r][:, ~sees].all() and not o[r][:, sees].isfinite().any(), r
+
+
+# (rows of each group) of calls whose groups are very unlike
+UNLIKE = [(64,) + (1,) * 256, (1000,) + (1,) * 1000, (1, 1, 300, 2, 1) + (3,) * 100]
+
+
+@pytest.mark.parametrize("sizes", UNLIKE)
+@pytest.mark.parametrize("H,KV,D", [(32, 8, 128), (4, 1, 64), (16, 16, 64)])
+def test_scratch_goes_by_the_rows_and_not_by_the_largest_group(sizes, H, KV, D):
+    """Prefix pieces take at most four copies of every row (one in float32), tails the same, and each of a few hundred blocks one piece more of 128 rows (32)."""
+    from mini_inference_b200.ops import load_calls
+    lib, R = load_calls(), sum(sizes)
+    for entry, copies, tile in ((lib.mi_attn_shared_tc_bytes, 4, 128), (lib.mi_attn_shared_f32_bytes, 1, 32)):
+        size = entry(R, len(sizes), max(sizes), H, KV, D, 16)
+        blocks = 2 * 160
+        assert 0 < size <= (2 * copies * R * H + 2 * blocks * tile) * (4 * D + 8) + 64 * R + 8192
+        assert size <= 2 ** 31                                     # (the largest of these took 15.7 GB when every group had the room of the largest)
+
+
+@gpu
+@pytest.mark.parametrize("sizes", UNLIKE)
+@pytest.mark.parametrize("H,KV,D,dtype", [(4, 1, 64, BF16), (8, 2, 128, BF16), (4, 1, 64, F32)])
+def test_groups_unlike_one_another(ops, sizes, H, KV, D, dtype):      # noqa: F811
+    groups = [(32 if n > 1 else 0, [33 + 5 * (i % 7) if i % 11 else 20 + i % 11 for i in range(n)]) for n in sizes]
+    q, k, v, meta = problem(groups, H, KV, D, 16, dtype, seed=sum(sizes))
+    check(ops, q, k, v, meta, H, KV, D)
