@@ -2,7 +2,7 @@
 
 The reference decodes greedily or by temperature only (engine/core/sampler.py:3-11); it has no counterpart of this.  A step
 feeds every beam its newest token (one entry each), picks every prompt's best candidates over its beams and the vocabulary on the device
-(CudaOps.beam_select) and reads them back: twice as many as beams, so that enough go on when some end.  The beams that go on take
+(CudaOps.beam_select) and reads them back: twice as many as beams, more with several end-of-sequence tokens, so that enough go on when some end.  The beams that go on take
 over their parents' caches (CacheManager.reorder): full pages by reference, the last page and recurrent states by one copy in place.  Attention over
 full contexts reads what all beams of a prompt share once (CudaOps.shared_prefix_attention)."""
 from __future__ import annotations
@@ -16,7 +16,8 @@ import torch
 from .batch import StepEntry
 from .runner import CacheFull
 
-MAX_BEAMS = 64                     # twice as many candidates are selected, at most 128
+MAX_BEAMS = 64
+MAX_CANDIDATES = 128               # that beam_select gives a group (CudaOps.MAX_CANDIDATES)
 
 
 @dataclass
@@ -197,10 +198,14 @@ class BeamSearch:
         starts = [0]
         for g in live:
             starts.append(starts[-1] + len(g.scores))
-        num = 2 * live[0].params.num_beams
+        # each of n beams can end in any of e ways: with n more candidates, n go on whatever ends
+        n, ends = live[0].params.num_beams, sum(0 <= t < logits.shape[1] for t in live[0].eos_ids)
+        num, bounds = n * max(2, 1 + ends), starts
+        if num > MAX_CANDIDATES:   # of every beam by itself, n and e hold as many that count; they are put in order here, equal values by the lower beam
+            num, bounds = n + ends, list(range(starts[-1] + 1))
         dev = logits.device
         host = torch.tensor([s for g in live for s in g.scores], dtype=torch.float32)
-        start = torch.tensor(starts, dtype=torch.int32)
+        start = torch.tensor(bounds, dtype=torch.int32)
         if dev.type == "cuda":
             host, start = host.pin_memory(), start.pin_memory()
         values, rows, tokens = self.ops.beam_select(logits, host.to(dev, non_blocking=True), start.to(dev, non_blocking=True), num)
@@ -208,6 +213,9 @@ class BeamSearch:
         values, rows, tokens = out[0].view(torch.float32).tolist(), out[1].tolist(), out[2].tolist()
         moves = []
         for i, g in enumerate(live):
-            found = [(v, r - starts[i], t) for v, r, t in zip(values[i], rows[i], tokens[i]) if r >= 0]
+            lists = range(starts[i], starts[i + 1]) if bounds is not starts else (i,)
+            found = [(v, r - starts[i], t) for k in lists for v, r, t in zip(values[k], rows[k], tokens[k]) if r >= 0]
+            if len(lists) > 1:
+                found.sort(key=lambda c: -c[0])               # stable: lower beams first
             moves.append((g, g.advance(found)))
         return moves

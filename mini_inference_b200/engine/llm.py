@@ -17,7 +17,7 @@ from ..cache.manager import CacheManager
 from ..config.engine_args import EngineArgs
 from ..sampling.sampler import Sampler
 from .batch import StepEntry
-from .beam import Beam, BeamParams, BeamSearch
+from .beam import MAX_CANDIDATES, Beam, BeamParams, BeamSearch
 from .factory import DTYPES, load_model
 from .request import RUNNING, Request, SamplingParams
 from .runner import ModelRunner
@@ -298,7 +298,7 @@ class LLM:
 
     def beam_search(self, prompts: Sequence[Sequence[int]], params: Optional[BeamParams] = None) -> List[List[Beam]]:
         """Token ids in; per prompt its num_beams best continuations, best first.  Runs by itself: requests that were added by add_request come first.  A prompt
-        whose beams do not fit beside one another in the cache raises CacheFull."""
+        whose beams do not fit beside one another in the cache raises CacheFull.  Beams and end-of-sequence tokens, where there are several, are at most 128 together."""
         if self.has_work():
             raise RuntimeError("beam_search runs by itself: step() until has_work() is False")
         params = params or BeamParams(max_new_tokens=self.args.max_new_tokens)
@@ -309,6 +309,9 @@ class LLM:
                 raise ValueError(f"prompt is {len(p)} tokens and {params.max_new_tokens} more are wanted; the limit is {limit}")
         if params.num_beams > self.args.max_num_seqs:
             raise ValueError(f"{params.num_beams} beams; the engine holds {self.args.max_num_seqs} sequences")
+        ends = 0 if params.ignore_eos else sum(0 <= t < self.model.spec.vocab_size for t in self.eos_ids)
+        if ends > 1 and params.num_beams + ends > MAX_CANDIDATES:
+            raise ValueError(f"{params.num_beams} beams and {ends} end-of-sequence tokens; at most {MAX_CANDIDATES} together are possible")
         with torch.inference_mode():
             out = BeamSearch(self).run(ids, params)
         if hasattr(self.ops, "check_errors"):
