@@ -7,7 +7,8 @@
 //
 // The order of two candidates is a whole number, so values are compared in float64 and the sum of exponentials is kept to about 1e-9: float32's 1e-7
 // would swap two neighbours that lie 0.05 apart once in some hundred thousand pairs, a step of 64 beams has a thousand.  Within a row the logits
-// themselves decide, exactly.
+// themselves decide, exactly.  Scores come in float32, so a caller with long sums gives what each row is behind its group's best one (as engine/beam.py does): a
+// number common to all rows of a group changes no order, and -800 in float32 is off by 3e-5.
 //
 // Two launches.  beam_slice_kernel: a block streams a slice of one row once (asynchronous copies, up to three tiles in front) and keeps its sum of exponentials and, per
 // thread, the largest logit.  The num / 8-th largest of each warp's 32 threads, the least of the eight, is a bound that num threads reach; the num-th of those that do is a

@@ -204,7 +204,9 @@ class BeamSearch:
         if num > MAX_CANDIDATES:   # of every beam by itself, n and e hold as many that count; they are put in order here, equal values by the lower beam
             num, bounds = n + ends, list(range(starts[-1] + 1))
         dev = logits.device
-        host = torch.tensor([s for g in live for s in g.scores], dtype=torch.float32)
+        # float32 holds what beams are behind their prompt's best one, not a long search's sums: those are kept in 64 bits, here
+        tops = [max(g.scores) for g in live]
+        host = torch.tensor([s - top for g, top in zip(live, tops) for s in g.scores], dtype=torch.float32)
         start = torch.tensor(bounds, dtype=torch.int32)
         if dev.type == "cuda":
             host, start = host.pin_memory(), start.pin_memory()
@@ -214,7 +216,7 @@ class BeamSearch:
         moves = []
         for i, g in enumerate(live):
             lists = range(starts[i], starts[i + 1]) if bounds is not starts else (i,)
-            found = [(v, r - starts[i], t) for k in lists for v, r, t in zip(values[k], rows[k], tokens[k]) if r >= 0]
+            found = [(tops[i] + v, r - starts[i], t) for k in lists for v, r, t in zip(values[k], rows[k], tokens[k]) if r >= 0]
             if len(lists) > 1:
                 found.sort(key=lambda c: -c[0])               # stable: lower beams first
             moves.append((g, g.advance(found)))

@@ -1853,7 +1853,8 @@ class CudaOps:
         candidate (row, token) has the value score + log_softmax(logits[row])[token].  Returns (values float32, rows int32, tokens int32), each [G, num]
         (num at most 128): the best of each group, best first; equal values: the lower row, then the larger logit, then the lower token.  Values are
         compared in float64.  Tokens with a logit of -inf are no candidates, nor are rows whose logits hold NaN or +inf or nothing finite or whose
-        score is not finite; places that stay empty hold (-inf, -1, -1)."""
+        score is not finite; places that stay empty hold (-inf, -1, -1).  Scores are exact to float32's rounding: long sums are best given as differences from their
+        group's largest, which changes no order."""
         here = self._device_index
         if (logits.dtype is not torch.float32 or scores.dtype is not torch.float32 or group_start.dtype is not torch.int32 or len(logits.shape) != 2 or scores.dim() != 1
                 or group_start.dim() != 1 or not scores.is_contiguous() or not group_start.is_contiguous() or scores.shape[0] != logits.shape[0]
