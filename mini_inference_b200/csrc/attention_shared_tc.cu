@@ -180,7 +180,7 @@ attn_shared_tc_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_con
     // Piece i, once it is found; false behind the last one (or with a wait that ran out).  Warp 0 is at most four pieces in front of all who read them: it waits
     // for the queries' rows of the piece before last, whose scores wait for the weights of the tile before last.
     const auto piece_at = [&](int i, Piece& piece) {
-        if (!mbar_wait(found + 8 * (i % PIECES), (i / PIECES) & 1)) { atomicExch(error_word, 59); return false; }
+        if (!mbar_wait(found + 8 * (i % PIECES), (i / PIECES) & 1)) { atomicExch(error_word, 101); return false; }
         const int4* from = reinterpret_cast<const int4*>(pieces + i % PIECES);
         int4* to = reinterpret_cast<int4*>(&piece);
         to[0] = from[0]; to[1] = from[1]; to[2] = from[2];
@@ -219,7 +219,7 @@ attn_shared_tc_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_con
         for (int n = 0, piece = 0; more; ++n) {
             const int s = n & 1;
             if (lane == 0) {
-                if (n >= 2 && !mbar_wait(empty + 8 * s, ((n >> 1) - 1) & 1)) { atomicExch(error_word, 61); ok = false; }
+                if (n >= 2 && !mbar_wait(empty + 8 * s, ((n >> 1) - 1) & 1)) { atomicExch(error_word, 103); ok = false; }
                 if (ok) mbar_expect_tx(full + 8 * s, KV_BYTES);
             }
             ok = __shfl_sync(0xffffffffu, ok, 0);
@@ -233,7 +233,7 @@ attn_shared_tc_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_con
                 const int rows = at.rows * Hg, copies = copies_of(1, rows), apart = BQ / copies, off = rows <= 16 && piece & 1 ? 16 : 0;
                 if (piece >= 2) ok = mbar_wait(q_done + 8 * (piece & 1), ((piece >> 1) - 1) & 1);
                 if (ok && piece && (rows > 16 || before > 16)) ok = mbar_wait(q_done + 8 * ((piece - 1) & 1), ((piece - 1) >> 1) & 1);
-                if (!__all_sync(0xffffffffu, ok)) { if (lane == 0) atomicExch(error_word, 60); break; }
+                if (!__all_sync(0xffffffffu, ok)) { if (lane == 0) atomicExch(error_word, 102); break; }
                 before = rows;
                 if (lane == 0) mbar_expect_tx(q_full + 8 * (piece & 1), rows * copies * D * 2);
                 __syncwarp();
@@ -261,7 +261,7 @@ attn_shared_tc_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_con
             bool more_s = piece_at(0, at), more_o = more_s;
             int tiles_s = at.tiles, tiles_o = at.tiles;
             for (uint32_t spins = 0; more_o; ++spins) {
-                if (spins == SPIN_LIMIT << 4) { atomicExch(error_word, 63); break; }
+                if (spins == SPIN_LIMIT << 4) { atomicExch(error_word, 105); break; }
                 if (more_s && tiles_s == 0 && mbar_test(found + 8 * (piece_s % PIECES), (piece_s / PIECES) & 1)) {
                     tiles_s = pieces[piece_s % PIECES].tiles;
                     more_s = tiles_s > 0;
@@ -321,7 +321,7 @@ attn_shared_tc_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_con
             for (int i = 0; i < tiles && ok; ++i, ++n) {
                 const int s = n & 1, key = at.key0 + i * KT;
                 const uint32_t s_addr = lane_addr + S_COL + 64 * s;
-                if (!mbar_wait(s_full + 8 * s, (n >> 1) & 1)) { atomicExch(error_word, 68); ok = false; break; }
+                if (!mbar_wait(s_full + 8 * s, (n >> 1) & 1)) { atomicExch(error_word, 106); ok = false; break; }
                 tc_fence_after();
                 float alpha = 1.f;
                 bool rescale = false;
@@ -333,7 +333,7 @@ attn_shared_tc_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_con
                 }
                 if (key < lo || key + KT > hi) {
                     // Values in front of the piece's first or behind its last key may be anything (a page's unused part), and 0 * inf is no 0
-                    if (!mbar_wait(v_full + 8 * s, (n >> 1) & 1)) { atomicExch(error_word, 62); ok = false; break; }
+                    if (!mbar_wait(v_full + 8 * s, (n >> 1) & 1)) { atomicExch(error_word, 104); ok = false; break; }
                     unsigned char* v = base + Q_BYTES + 2 * KV_BYTES + s * KV_BYTES;
                     const int box = min(a.ps, KT), first = max(0, lo - key), last = min(KT, hi - key), end = min(KT, (last + box - 1) / box * box);
                     for (int id = tid; id < (first + end - last) * HALVES * 8; id += 128) {
@@ -343,7 +343,7 @@ attn_shared_tc_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_con
                     asm volatile("fence.proxy.async.shared::cta;\n" ::: "memory");
                 }
                 // every thread follows pv_done phase by phase; O holds the tile before this one completely after it
-                if (n > 0 && !mbar_wait(pv_done, (n - 1) & 1)) { atomicExch(error_word, 69); ok = false; }
+                if (n > 0 && !mbar_wait(pv_done, (n - 1) & 1)) { atomicExch(error_word, 107); ok = false; }
                 if (__any_sync(0xffffffffu, rescale)) {
                     tc_fence_after();
 #pragma unroll 1
@@ -361,7 +361,7 @@ attn_shared_tc_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_con
                 mbar_arrive(p_ready);
             }
             if (!ok) break;
-            if (!mbar_wait(pv_done, (n - 1) & 1)) { atomicExch(error_word, 70); break; }
+            if (!mbar_wait(pv_done, (n - 1) & 1)) { atomicExch(error_word, 108); break; }
             tc_fence_after();
             if (active) {
                 const int rows_of = copies * rows, line = copy * rows + mine;
