@@ -12,6 +12,7 @@ from __future__ import annotations
 import array
 import ctypes
 import math
+import operator
 import os
 import types
 
@@ -1887,15 +1888,32 @@ class CudaOps:
             raise ValueError(f"beam_select: {num} candidates a group, between 1 and {self.MAX_CANDIDATES} are possible")
         self._here("beam_select", logits=logits, scores=scores, group_start=group_start)
 
+    @staticmethod
+    def _overlap(places):
+        """Whether rows of two tensors (places as reorder_rows makes them) share a byte.  Tensors that reach into one another do not where one's rows lie between the
+        other's: exact for rows of one distance, and refused in doubt for rows of two."""
+        spans = []                                   # address, end, bytes from row to row (0: one piece), bytes of a row
+        for a, lead, table, _, stride, row in zip(*(places[i::6] for i in range(6))):
+            if lead * table * row:
+                spans.append((a, a + lead * table, 0, lead * table) if row == stride else (a, a + table - stride + row, stride, row))
+        spans.sort()
+        for i, (a, a_end, a_stride, a_row) in enumerate(spans):
+            for b, _, b_stride, b_row in spans[i + 1:]:
+                if b >= a_end:
+                    break
+                step = math.gcd(a_stride, b_stride)
+                off = (b - a) % step if step else 0  # how far behind the beginning of a's row b's begin
+                if off < a_row or off + b_row > step:
+                    return True
+        return False
+
     def reorder_rows(self, tensors, rows, parents, group_start, most, dim=0):
         """In place, for every tensor t of `tensors` and every i: t[rows[i]] = what t[rows[parents[i]]] was before the call (a beam takes over its parent's
         state).  dim: which dimension of the tensors the rows are (those before it are as many tables with the same rows; tensors of any type, contiguous
         from the rows' dimension on, and before it too).  rows, parents int32 [n]; group_start int32 [G + 1]: places group_start[g] .. group_start[g + 1] - 1 of
-        both lists are a group, parents (places in the lists) lie in their row's group; most: rows of the largest group, at most 100.  A row is named once, no
-        tensor twice.  A parent outside its group, or a row that a tensor does not have, leaves the row as it is."""
+        both lists are a group, parents (places in the lists) lie in their row's group; most: rows of the largest group, at most 100.  A row is named once, and
+        the tensors share no memory (columns of one wider tensor may be several of them).  A parent outside its group, or a row that a tensor does not have, leaves the row as it is."""
         tensors, here = list(tensors), self._device_index
-        if len(set(map(torch.Tensor.data_ptr, tensors))) < len(tensors) and len({t.data_ptr() for t in tensors if t.numel()}) < sum(t.numel() > 0 for t in tensors):
-            raise ValueError("reorder_rows: two of the tensors are the same memory")
         if (not (rows.dtype is parents.dtype is group_start.dtype is torch.int32) or not (rows.is_contiguous() and parents.is_contiguous() and group_start.is_contiguous())
                 or rows.dim() != 1 or rows.shape != parents.shape or group_start.dim() != 1 or group_start.shape[0] < 1 or not 0 <= most <= self.MAX_BEAMS):
             self._plain("reorder_rows", torch.int32, rows=rows, parents=parents, group_start=group_start)
@@ -1916,6 +1934,10 @@ class CudaOps:
                 if dim or not t[:1].is_contiguous() or stride < row:
                     raise ValueError(f"reorder_rows: a tensor of shape {tuple(shape)} has strides {t.stride()} (rows lie in one piece)")
             places.extend((t.data_ptr(), lead, n * stride, n, stride, row))
+        if len(tensors) > 1:                         # each ends in front of the next one's begin, or a closer look
+            ends = [a + lead * table for a, lead, table in zip(places[0::6], places[1::6], places[2::6])]
+            if any(map(operator.gt, sorted(ends), sorted(places[0::6])[1:])) and self._overlap(places):
+                raise ValueError("reorder_rows: two of the tensors are the same memory")
         if not rows.get_device() == parents.get_device() == group_start.get_device() == here or any(t.get_device() != here for t in tensors):
             self._here("reorder_rows", rows=rows, parents=parents, group_start=group_start, **{f"tensor {i}": t for i, t in enumerate(tensors)})
         if not tensors:
