@@ -54,11 +54,11 @@ class SeqCache:
 
 
 class Family:
-    """What the beams of one prompt have in common: the first `shared` tokens lie on the same pages in every group that keeps all keys."""
-    __slots__ = ("shared",)
+    """What the beams of one prompt have in common: the first `shared` tokens of all that live lie on the same pages in every group that keeps all keys."""
+    __slots__ = ("shared", "members")
 
-    def __init__(self):
-        self.shared = 0
+    def __init__(self, first):
+        self.shared, self.members = 0, [first]
 
 
 class _Group:
@@ -251,6 +251,8 @@ class CacheManager:
                 g.dirty[base + idx] = None
         self.slots.release(seq.slot)
         del self.seqs[seq.seq_id]
+        if seq.family is not None:
+            seq.family.members.remove(seq)
 
     # ---------------------------------------------------------------- beams
     def fork(self, seq: SeqCache, seq_ids) -> Optional[List[SeqCache]]:
@@ -262,7 +264,7 @@ class CacheManager:
         if self.slots.num_free < len(seq_ids) or (part and any(g.pool.num_free < len(seq_ids) for g in self.kv_groups)):
             return None
         if seq.family is None:
-            seq.family = Family()
+            seq.family = Family(seq)
         children = []
         for i in seq_ids:
             child = SeqCache(i, self.slots.claim(), len(self.kv_groups))
@@ -278,23 +280,25 @@ class CacheManager:
                     self._set_entry(g, child.slot, idx, page)
             self.seqs[i] = child
             children.append(child)
-        self._measure_family([seq, *children])
+        seq.family.members += children
+        self._measure(seq.family)
         return children
 
     def _set_entry(self, g: _Group, slot: int, idx: int, page: int) -> None:
         g.tables[slot, idx] = page
         g.dirty[slot * self.max_pages_per_seq + idx] = None
 
-    def _measure_family(self, seqs) -> None:
+    def _measure(self, family: Family) -> None:
         """How many leading tokens lie on common pages."""
-        full = seqs[0].num_tokens // self.page_size
+        seqs = family.members
+        full = min(s.num_tokens for s in seqs) // self.page_size
         whole = next((g for g in self.kv_groups if g.need.window is None), None)
         same = 0
         if whole is not None and full:
             rows = whole.tables[[s.slot for s in seqs], :full]
             differ = (rows != rows[0]).any(axis=0)
             same = int(differ.argmax()) if differ.any() else full
-        seqs[0].family.shared = same * self.page_size
+        family.shared = same * self.page_size
 
     def reorder(self, groups, ops) -> None:
         """groups: [(beams of one prompt, a parent's place among them for each)].  Every beam then holds what its parent held.  The beams of a prompt
@@ -320,7 +324,7 @@ class CacheManager:
                 if part:
                     self._add_move(moves[gi], [int(g.tables[s.slot, full]) for s in seqs], parents)
             self._add_move(moves[-1], [s.slot for s in seqs], parents)
-            self._measure_family(seqs)
+            self._measure(seqs[0].family)
         tensors = [[(g.storage, 2)] + ([(g.value_storage, 1)] if g.value_storage is not None else []) for g in self.kv_groups]
         tensors.append([(g.storage, 0) for g in self.state_groups])
         for (rows, parents, start), held in zip(moves, tensors):
