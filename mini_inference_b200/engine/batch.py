@@ -26,6 +26,7 @@ and drops those of unfinished prompts (engine/custom_engine.py:139,155-157)."""
 from __future__ import annotations
 
 import os
+from collections import Counter
 from typing import Dict, List, Optional, Sequence
 
 import numpy as np
@@ -118,8 +119,10 @@ class StepBatch:
         self.max_kv_len, self.max_q_len = max_kv_len, int(facts.lens.max())
         prompts = facts.lens > 1                                    # entries that feed more than one token; the most keys one of them sees
         self.max_prompt_kv_len = int(facts.kv_len[prompts].max()) if prompts.any() else 0
-        groups = [0] if facts.shared is None else np.unique([g for g, _ in facts.shared], return_counts=True)[1]
-        self.max_shared_rows = int(max(groups))
+        # rows of the largest group of beams, the longest prefix that several rows share
+        groups = Counter(facts.shared or ())
+        self.max_shared_rows = max(groups.values(), default=0)
+        self.max_shared_len = max((n for (_, n), rows in groups.items() if rows > 1), default=0)
         self.host = {"seg_q_start": facts.q_start, "seg_pos0": facts.pos0, "seg_kv_len": facts.kv_len,
                      "seg_slot": facts.slots.tolist(), "lens": facts.lens}
         for name in ("token_ids", "positions", "token_seg", "seg_q_start", "seg_pos0", "seg_kv_len", "seg_slot", "logit_rows"):

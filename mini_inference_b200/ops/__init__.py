@@ -666,7 +666,8 @@ class CudaOps:
         block_table and table_rows as paged_attention reads them (max_kv_len: the longest); shared_start int32 [G + 1]: entries decode_segs[shared_start[g]] ..
         decode_segs[shared_start[g + 1] - 1] are group g (rows in no group stand alone), shared_len int32 [G]: the first so many keys of its rows are the
         same, and are read by the pages of the first row that has them all (a row that has fewer is computed by its own pages); max_shared_rows, on the host: rows of the largest
-        group (rows beyond it are computed alone).  An entry without keys gets zeros.  The output [T, H D] has the entries' rows; others are left as they come.  What lies behind
+        group (rows beyond it are computed alone); max_shared_len, on the host, may say the longest shared length (of groups of several rows): float32 calls
+        that share little are then computed row by row, which is faster.  An entry without keys gets zeros.  The output [T, H D] has the entries' rows; others are left as they come.  What lies behind
         an entry's keys counts for nothing; NaN among the keys and queries that it sees makes it NaN, and a value that is not finite makes its column not finite.
         Heads of 64 or 128 run on kernels that share; other heads, more than 4,096 entries and groups, bfloat16 pages that neither divide 64 keys nor are divided
         by them, bfloat16 rows that do not lie whole heads apart, and calls that read little (SHARED_BYTES) are computed row by row, by the rows' own pages."""
@@ -753,12 +754,20 @@ class CudaOps:
     # What the rows would read one by one, from which on sharing is the faster way: less stays in the L2 cache from one row to the next, and one launch does for it.
     # Microseconds, sharing / one by one, 32 heads over 8 of 128.  bfloat16: 4 rows x 512 keys 15 / 8, 16 x 1,024 (69 MB) 18 / 17, 8 x 2,048 (68 MB) 22 / 17, 8 x 4,096
     # (135 MB) 25 / 26, 16 x 2,048 (136 MB) 19 / 26, 8 groups of 4 x 1,024 (138 MB) 24 / 25, 8 x 8 x 1,024 (277 MB) 30 / 47, 8 x 8 x 4,096 46 / 157.  float32, whose
-    # multiply-adds bound the shared form: 13 rows x 1,600 (171 MB) 37 / 31, 8 x 4,096 (270 MB) 44 / 44, 8 x 8 x 512 (285 MB) 75 / 49, 16 x 4,096 (541 MB) 68 / 78, 8 x
-    # 16 x 512 (570 MB) 126 / 97, 8 x 8 x 2,048 (1.1 GB) 137 / 175.
+    # multiply-adds bound the shared form: 13 rows x 1,600 (171 MB) 37 / 31, 8 x 4,096 (270 MB) 44 / 44, 8 x 8 x 512 (285 MB) 75 / 49, 16 x 4,096 (541 MB) 68 / 78, 8 x 8 x
+    # 2,048 (1.1 GB) 137 / 175.  It is no rule for many short prefixes, which stay in L2: 4 x 16 x 1,024 (545 MB) 92 / 79, 8 x 16 x 512 (570 MB) 126 / 97.
     SHARED_BYTES = {torch.bfloat16: 128 << 20, torch.float32: 512 << 20}
+    # ... and how much of the longest row the longest shared prefix is at least, where the host says so (max_shared_len).  float32 tails fill an eighth of a tile's rows and
+    # cost as much: 8 x 8 rows, 2,048 shared keys and 128, 256, 1,024 own ones 168 / 186, 209 / 197, 448 / 271; 16 x 4,096 and 16, 256, 512 68 / 78, 86 / 83, 106 / 103; 64 rows
+    # of 2,048, 64 shared, 436 / 211.  bfloat16 loses little where nothing is shared (64 x 2,048 95 / 89, 16 x 4,096 54 / 47) and gains in rows unlike one another, whose tiles
+    # it shares out evenly (one of 8,192 and 15 of 256 27 / 66, and 63 of 256 37 / 133), so it is not asked.
+    SHARED_PART = {torch.bfloat16: 0.0, torch.float32: 0.9}
 
     def _sharing_pays(self, q, meta, KV, D, bf16):
-        return len(meta.decode_segs) * meta.max_kv_len * KV * D * (4 if bf16 else 8) > self.SHARED_BYTES[q.dtype]
+        if len(meta.decode_segs) * meta.max_kv_len * KV * D * (4 if bf16 else 8) <= self.SHARED_BYTES[q.dtype]:
+            return False
+        shared = getattr(meta, "max_shared_len", None)
+        return shared is None or shared >= self.SHARED_PART[q.dtype] * meta.max_kv_len
 
     def _shared_bytes(self, q, k_cache, v_cache, meta, H, KV, D):
         """Bytes of scratch of the kernel that reads shared prefixes once; not above 0: these rows are computed one by one."""
