@@ -619,7 +619,7 @@ class CudaOps:
             self.launches += 1
         if not num_decode:
             return out
-        if not win and not split_weights and getattr(meta, "shared_start", None) is not None and self._sharing_pays(q, meta, KV, D, q.dtype is torch.bfloat16):
+        if not win and not split_weights and scale > 0 and getattr(meta, "shared_start", None) is not None and self._sharing_pays(q, meta, KV, D, q.dtype is torch.bfloat16):
             size = self._shared_bytes(q, k_cache, v_cache, meta, H, KV, D)
             if size > 0:
                 self._shared_decode(q, k_cache, v_cache, out, meta, H, KV, D, scale, size)

@@ -1,10 +1,12 @@
 """Which decode steps go to the kernels that share prefixes: the rule on the host, and what a step of beams tells it."""
 import types
 
+import pytest
 import torch
 
 from mini_inference_b200.engine.batch import BatchBuilder, StepEntry, shared_of
 from mini_inference_b200.cache import CacheManager
+from mini_inference_b200.ops import CudaOps
 from mini_inference_b200.parts.attention import paged_attention_step_arrays
 from mini_inference_b200.parts.base import KVCacheNeed
 from tests.ref_beam import BeamRefOps
@@ -75,3 +77,20 @@ def test_what_a_step_of_beams_says():
     assert step(a[0], prompt, a[1], a[2], portion=(prompt,)) == ([0, 1, 3], [20, 20], 2, 20)
     assert step(other, prompt)[2:] == (0, 0) and step(other, prompt)[0] is None
     assert shared_of([other, prompt], [1, 1]) is None
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [BF16, F32])
+def test_paged_attention_with_a_scale_below_zero(monkeypatch, dtype):
+    """paged_attention takes any scale; the kernels that share take the largest product for the largest score, which asks for a positive one."""
+    from mini_inference_b200.ops import get_ops
+    from tests.test_shared_attention import check, problem
+    ops = get_ops("cuda:0")
+    monkeypatch.setattr(CudaOps, "SHARED_BYTES", {BF16: 0, F32: 0})
+    q, k, v, meta = problem([(160, [161, 200, 300]), (64, [65, 90])], 8, 2, 128, 16, dtype, seed=4)
+    q = (q.float() * 12).to(dtype)                                 # products of some hundred: their weights by the wrong end overflow
+    meta.prefill_tiles, meta.tile = meta.decode_segs[:0].view(0, 2), 64
+    got = ops.paged_attention(q, k, v, meta, 8, 2, 128, -1.0, None)
+    check(ops, -q, k, v, meta, 8, 2, 128, scale=1.0, got=got)      # the same scores, exactly
+    got = ops.paged_attention(q, k, v, meta, 8, 2, 128, 1.0, None)
+    check(ops, q, k, v, meta, 8, 2, 128, scale=1.0, got=got)
