@@ -16,6 +16,7 @@
 // A group of one row has no prefix part: its whole length is its tail.
 #pragma once
 #include "common.cuh"
+#include <atomic>
 
 namespace mi {
 namespace shared_attention {
@@ -305,13 +306,13 @@ template <typename T, int D> inline cudaError_t merge(const Args& a, T* out, cud
     return launch_pdl(merge_kernel<T, D, 2>, dim3(a.R, a.KV), dim3(256), 0, stream, a, out);
 }
 
-// Lets a kernel have `bytes` of shared memory, once a device (asking again costs a call about 2 us)
-template <typename Kernel> inline cudaError_t allow_shared(Kernel kernel, int bytes, unsigned long long& devices_done) {
+// Lets a kernel have `bytes` of shared memory, once a device (asking again costs a call about 2 us).  Calls of several host threads may meet here.
+template <typename Kernel> inline cudaError_t allow_shared(Kernel kernel, int bytes, std::atomic<unsigned long long>& devices_done) {
     int dev = 0;
     cudaError_t e = cudaGetDevice(&dev);
-    if (e != cudaSuccess || (dev < 64 && devices_done >> dev & 1)) return e;
+    if (e != cudaSuccess || (dev < 64 && devices_done.load() >> dev & 1)) return e;
     e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
-    if (e == cudaSuccess && dev < 64) devices_done |= 1ull << dev;
+    if (e == cudaSuccess && dev < 64) devices_done.fetch_or(1ull << dev);
     return e;
 }
 

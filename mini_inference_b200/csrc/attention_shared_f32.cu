@@ -200,7 +200,7 @@ MI_EXPORT int mi_attn_shared_f32(const float* q, int q_stride, const float* k_ca
     const float scale_log2 = scale * 1.4426950408889634f;
 #define LAUNCH(DD) do { \
         const size_t smem = (size_t)Tiles<DD>::END * 4, plan = (size_t)plan_ints(G, R) * 4; \
-        static unsigned long long done = 0; \
+        static std::atomic<unsigned long long> done{0}; \
         cudaError_t e = allow_shared(attn_shared_f32_kernel<DD>, (int)(smem + (6 * MAX_ENTITIES + 1) * 4), done); \
         if (e == cudaSuccess) e = launch_pdl(attn_shared_f32_kernel<DD>, dim3(blocks), dim3(THREADS), smem + plan, stream, a, q, (long long)q_stride, k_cache, v_cache, \
                                              scale_log2); \

@@ -388,6 +388,8 @@ attn_shared_tc_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_con
     if (warp == 1) tmem_dealloc(tmem, TMEM_COLS);
 }
 
+// Maps of the caches that calls came with: addresses and shapes.  An engine has a few; a program that makes caches over and over begins again from none.
+constexpr size_t MAPS = 1024;
 std::mutex map_mutex;
 std::map<std::tuple<const void*, long long, int, int>, CUtensorMap> maps;
 
@@ -398,6 +400,7 @@ bool cache_map(const void* cache, long long rows, int D, int box, CUtensorMap* o
     if (it == maps.end()) {
         CUtensorMap m;
         if (!sm100_host::make_map_bf16(&m, cache, (uint64_t)rows, D, D, box, 64)) return false;
+        if (maps.size() >= MAPS) maps.clear();
         it = maps.emplace(key, m).first;
     }
     *out = it->second;
@@ -462,7 +465,7 @@ MI_EXPORT int mi_attn_shared_tc(const void* q, int q_stride, int tokens, const v
     const size_t smem = bytes(plan_ints(G, R)), most_smem = bytes(6 * MAX_ENTITIES + 1);
     const float scale_log2 = scale * LOG2E;
 #define LAUNCH(DD) do { \
-        static unsigned long long done = 0; \
+        static std::atomic<unsigned long long> done{0}; \
         cudaError_t e = allow_shared(attn_shared_tc_kernel<DD>, (int)most_smem, done); \
         if (e == cudaSuccess) e = launch_pdl(attn_shared_tc_kernel<DD>, dim3(blocks), dim3(THREADS), smem, stream, qmap, kmap, vmap, a, scale_log2, error_word); \
         if (e == cudaSuccess) e = merge<__nv_bfloat16, DD>(a, (__nv_bfloat16*)out, stream); \
