@@ -780,13 +780,13 @@ class CudaOps:
 
     def _shared_decode(self, q, k_cache, v_cache, out, meta, H, KV, D, scale, size):
         segs, kv_len, shared = meta.decode_segs, meta.seg_kv_len, meta.shared_len
+        stride = q.stride(0) if len(q) > 1 else H * D    # as _shared_bytes takes it
         rows = (out, segs, len(segs), meta.seg_q_start, kv_len, len(kv_len), meta.block_table, getattr(meta, "table_rows", None), meta.max_pages, meta.shared_start,
                 shared, len(shared), meta.max_shared_rows, H, KV, D, meta.page_size, scale, segs.new_empty((size + 3) // 4))
         if q.dtype is torch.bfloat16:
-            _check(self.lib.mi_attn_shared_tc(q, q.stride(0) if len(q) > 1 else H * D, len(q), k_cache, v_cache, k_cache.shape[0] * KV * meta.page_size, *rows, self._stream_error, self._stream()),
-                   "attn_shared_tc")
+            _check(self.lib.mi_attn_shared_tc(q, stride, len(q), k_cache, v_cache, k_cache.shape[0] * KV * meta.page_size, *rows, self._stream_error, self._stream()), "attn_shared_tc")
         else:
-            _check(self.lib.mi_attn_shared_f32(q, q.stride(0), k_cache, v_cache, *rows, self._stream()), "attn_shared_f32")
+            _check(self.lib.mi_attn_shared_f32(q, stride, k_cache, v_cache, *rows, self._stream()), "attn_shared_f32")
         self.launches += 2
 
     # Where split softmax weights run on tcgen05: a prompt portion sees (first) so many keys, or 256 in a step of (second) so many tokens.  On the

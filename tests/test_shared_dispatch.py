@@ -94,3 +94,18 @@ def test_paged_attention_with_a_scale_below_zero(monkeypatch, dtype):
     check(ops, -q, k, v, meta, 8, 2, 128, scale=1.0, got=got)      # the same scores, exactly
     got = ops.paged_attention(q, k, v, meta, 8, 2, 128, 1.0, None)
     check(ops, q, k, v, meta, 8, 2, 128, scale=1.0, got=got)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [BF16, F32])
+def test_one_token_in_a_row_of_any_width(monkeypatch, dtype):
+    """A single token has no distance to the next one, whatever its stride says."""
+    from mini_inference_b200.ops import get_ops
+    from tests.test_shared_attention import check, problem
+    ops = get_ops("cuda:0")
+    monkeypatch.setattr(CudaOps, "SHARED_BYTES", {BF16: 0, F32: 0})
+    q, k, v, meta = problem([(0, [300])], 8, 2, 64, 16, dtype, seed=4)
+    for width in (8 * 64 + 1, 8 * 64 + 3, 8 * 64 + 8):
+        wide = torch.randn(1, width, device=q.device).to(dtype)
+        check(ops, wide[:, :8 * 64], k, v, meta, 8, 2, 64)
+    check(ops, wide.as_strided((1, 8 * 64), (0, 1)), k, v, meta, 8, 2, 64)
