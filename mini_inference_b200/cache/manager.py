@@ -302,13 +302,20 @@ class CacheManager:
 
     def reorder(self, groups, ops) -> None:
         """groups: [(beams of one prompt, a parent's place among them for each)].  Every beam then holds what its parent held.  The beams of a prompt
-        have cached the same number of tokens."""
-        moves = [([], [], [0]) for _ in range(len(self.kv_groups) + 1)]        # per kv group, and for the states: rows, parents (places in rows), group starts
+        have cached the same number of tokens, and each is named once.  Nothing is changed where one of the groups is refused."""
+        groups = list(groups)
+        most, named = getattr(ops, "MAX_BEAMS", None), [id(s) for seqs, _ in groups for s in seqs]
+        if len(set(named)) < len(named):
+            raise RuntimeError("a beam takes over one cache: it is named twice")
         for seqs, parents in groups:
+            if most is not None and len(seqs) > most:
+                raise ValueError(f"{len(seqs)} beams of a prompt; at most {most} take over one another's cache")
             if len(seqs) != len(parents) or any(not 0 <= p < len(seqs) for p in parents):
                 raise ValueError(f"{len(parents)} parents {list(parents)!r} for {len(seqs)} beams")
             if any(s.num_tokens != seqs[0].num_tokens or s.family is not seqs[0].family or s.family is None or not s.alive for s in seqs):
                 raise RuntimeError("only beams of one prompt that have cached the same number of tokens take over one another's cache")
+        moves = [([], [], [0]) for _ in range(len(self.kv_groups) + 1)]        # per kv group, and for the states: rows, parents (places in rows), group starts
+        for seqs, parents in groups:
             if all(p == i for i, p in enumerate(parents)):
                 continue
             full, part = divmod(seqs[0].num_tokens, self.page_size)

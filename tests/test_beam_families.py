@@ -91,3 +91,31 @@ def test_at_random(seed):
         elif len(seqs) > 1:
             cache.free(seqs.pop(rng.randrange(len(seqs))))
         check(cache, seqs)
+
+
+class NoMoreThanFour(BeamRefOps):
+    MAX_BEAMS = 4
+
+    def reorder_rows(self, tensors, rows, parents, group_start, most, dim=0):
+        assert most <= 4
+        super().reorder_rows(tensors, rows, parents, group_start, most, dim)
+
+
+def test_a_refused_group_changes_nothing():
+    """... of the groups in front of it either."""
+    cache, seqs = family(4, 9)
+    grow(cache, seqs, 6)
+    other = cache.admit("other")
+    assert cache.ensure(other, 15)
+    cache.commit(other, 15)
+    more = [other] + cache.fork(other, [f"o{i}" for i in range(1, 6)])
+    before = [g.tables.copy() for g in cache.kv_groups], [list(g.pool.ref) for g in cache.kv_groups]
+    for bad, error in (([(seqs, [1, 1, 0, 0]), (more[:2], [0, 2])], ValueError), ([(seqs, [1, 1, 0, 0]), (more[:2], [0])], ValueError),
+                       ([(seqs, [1, 1, 0, 0]), ([other, seqs[0]], [0, 0])], RuntimeError), ([(seqs, [1, 1, 0, 0]), (more, [0] * 6)], ValueError),
+                       ([(seqs[:2], [1, 1]), (seqs[1:], [0, 0, 0])], RuntimeError), ([([seqs[0], seqs[0]], [1, 1])], RuntimeError)):
+        with pytest.raises(error):
+            cache.reorder(bad, NoMoreThanFour())
+        assert all((a == g.tables).all() for a, g in zip(before[0], cache.kv_groups)) and before[1] == [list(g.pool.ref) for g in cache.kv_groups]
+        cache.check_invariants()
+    cache.reorder(iter([(seqs, [1, 1, 0, 0]), (more[:4], [1, 1, 0, 0])]), NoMoreThanFour())
+    check(cache, seqs)
