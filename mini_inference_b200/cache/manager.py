@@ -335,6 +335,7 @@ class CacheManager:
         tensors = [[(g.storage, 2)] + ([(g.value_storage, 1)] if g.value_storage is not None else []) for g in self.kv_groups]
         tensors.append([(g.storage, 0) for g in self.state_groups])
         for (rows, parents, start), held in zip(moves, tensors):
+            held = [(t, dim) for t, dim in held if t is not None]              # (a cache without storage keeps tables only)
             if not rows or not held:
                 continue
             lists = torch.tensor(rows + parents + start, dtype=torch.int32)

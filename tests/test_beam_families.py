@@ -119,3 +119,16 @@ def test_a_refused_group_changes_nothing():
         cache.check_invariants()
     cache.reorder(iter([(seqs, [1, 1, 0, 0]), (more[:4], [1, 1, 0, 0])]), NoMoreThanFour())
     check(cache, seqs)
+
+
+def test_a_cache_without_storage():
+    """Tables and pages alone."""
+    cache = CacheManager([KVCacheNeed(2, 8), StateNeed((3,))], PS, 40, 8, 80, dtype=torch.float32, allocate=False)
+    a = cache.admit("a")
+    assert cache.ensure(a, 6)
+    cache.commit(a, 6)
+    seqs = [a] + cache.fork(a, ["b", "c"])
+    cache.reorder([(seqs, [0, 0, 0])], BeamRefOps())
+    grow(cache, seqs, 7)
+    cache.reorder([(seqs, [2, 2, 0])], BeamRefOps())
+    check(cache, seqs)
