@@ -32,8 +32,10 @@ class BeamParams:
             raise ValueError(f"{self.num_beams} beams: between 1 and {MAX_BEAMS} are possible")
         if self.max_new_tokens < 1:
             raise ValueError("max_new_tokens must be positive")
-        if not abs(self.length_penalty) <= 64:            # (a length to that power is still a float)
+        if not abs(self.length_penalty) <= 64:
             raise ValueError("length_penalty must be between -64 and 64")
+        if abs(self.length_penalty) * math.log(self.max_new_tokens) > 650:      # a rank divides a score by that power: both stay floats
+            raise ValueError(f"a length of {self.max_new_tokens} to the power of length_penalty ({self.length_penalty}) is no number")
 
 
 @dataclass

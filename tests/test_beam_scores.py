@@ -69,3 +69,15 @@ def test_the_engine_s_scores(tiny_dirs):
         lp = torch.log_softmax(llm.score(prompt + b.tokens).double(), -1)
         want = sum(float(lp[len(prompt) - 1 + i, t]) for i, t in enumerate(b.tokens))
         assert abs(b.score - want) <= 60 * (2.0 ** -20 + 1e-5)     # (a step's logits and the whole hypothesis' agree to 1e-5 or so)
+
+
+def test_lengths_whose_power_is_no_number_are_refused():
+    """A rank divides by a length to the power of length_penalty."""
+    for n, p in ((100000, 64.0), (100000, -64.0), (2 ** 31, 40.0), (10 ** 300, 1.5)):
+        with pytest.raises(ValueError, match="length_penalty"):
+            BeamParams(max_new_tokens=n, length_penalty=p)
+    for n, p in ((10000, 64.0), (10000, -64.0), (2 ** 20, 40.0), (2 ** 40, 1.0), (1, 64.0)):
+        g = BeamGroup([1], BeamParams(max_new_tokens=n, length_penalty=p, num_beams=1), {7})
+        g.tokens = [[3] * (n - 1 if n < 2 ** 21 else 10)]
+        g.advance([(-1e4, 0, 7)])
+        assert math.isfinite(g.ended[0].rank) and g.ended[0].rank < 0
