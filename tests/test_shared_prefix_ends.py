@@ -84,3 +84,13 @@ def test_groups_unlike_one_another(ops, sizes, H, KV, D, dtype):      # noqa: F8
     groups = [(32 if n > 1 else 0, [33 + 5 * (i % 7) if i % 11 else 20 + i % 11 for i in range(n)]) for n in sizes]
     q, k, v, meta = problem(groups, H, KV, D, 16, dtype, seed=sum(sizes))
     check(ops, q, k, v, meta, H, KV, D)
+
+
+@gpu
+@pytest.mark.parametrize("H,KV,D,ps,dtype", [(128, 1, 128, 16, BF16), (96, 2, 64, 16, BF16), (40, 1, 128, 16, BF16), (33, 1, 64, 32, BF16), (65, 1, 64, 256, BF16), (64, 64, 64, 16, BF16), (34, 2, 128, 16, BF16),
+                                             (32, 1, 64, 16, F32), (17, 1, 128, 8, F32), (21, 3, 64, 16, F32), (48, 48, 64, 1, F32)])
+def test_many_query_heads_of_a_key_head(ops, H, KV, D, ps, dtype):      # noqa: F811
+    """A row alone fills a tile, or half of one and a head more; many key heads."""
+    for groups in ([(256, [257, 300, 256, 12])], [(0, [700]), (64, [65 + 3 * i for i in range(9)])]):
+        q, k, v, meta = problem(groups, H, KV, D, ps, dtype, seed=H + KV)
+        check(ops, q, k, v, meta, H, KV, D)
