@@ -300,7 +300,7 @@ __global__ void __launch_bounds__(128 * PARTS, PARTS == 2 ? 4 : 1) merge_kernel(
     }
 }
 // Few rows leave SMs empty, and there eight groups of threads a row are the faster ones (16 rows of 8 key heads, 80 pieces each: 47 us for the
-// whole operator, with two groups 51); many rows want four blocks an SM (64 rows, 25 pieces: two groups 51 us, four 54).
+// whole operator, with two groups 58); many rows want four blocks an SM (8 x 8 rows on 4,096 keys: two groups 48 us, eight 56; 64 on 8,192: 53 and 61).
 template <typename T, int D> inline cudaError_t merge(const Args& a, T* out, cudaStream_t stream) {
     if ((long long)a.R * a.KV <= device_sms()) return launch_pdl(merge_kernel<T, D, 8>, dim3(a.R, a.KV), dim3(1024), 0, stream, a, out);
     return launch_pdl(merge_kernel<T, D, 2>, dim3(a.R, a.KV), dim3(256), 0, stream, a, out);

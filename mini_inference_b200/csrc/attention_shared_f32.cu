@@ -4,8 +4,8 @@
 // ends of pieces too; what lies outside the visible keys comes as zeros.  Scores: a thread has two rows and two keys (padded rows in shared memory, so that
 // 16 keys' pieces lie in different banks); softmax: eight threads a row, float32, base 2; weighted sums: a warp has four rows, a lane D / 32
 // neighbouring columns in registers.  Bound by shared-memory reads (six wavefronts for sixteen multiply-adds of a warp); a tail's few rows leave most warps
-// out, and there it is bound by the bytes.  13 rows in two groups on 1,504 and 976 shared and 100 own keys (32 heads over 8 of 128): 38 us with the merge (row by
-// row, as calls of that size run, 31); its
+// out, and there it is bound by the bytes.  13 rows in two groups on 1,504 and 976 shared and 100 own keys (32 heads over 8 of 128): 37 us with the merge (row by
+// row, as calls of that size run, 29); its
 // multiply-adds would take 4.  A block has three to five tiles then, and each piece's queries, page numbers and first keys come one behind the other.  Scores in
 // 4 x 4 squares over quarters of the head, and a warp per four keys for tails, took 36 us there and 8 % less at 8 x 2,048 keys, 8 % more for tails alone.
 #include "attention_shared.cuh"

@@ -22,8 +22,9 @@
 // Two launches: this one, and the merge.  Every mbarrier wait is bounded.
 //
 // Measured (32 query heads over 8 key heads of 128, pages of 16): 8 groups of 8 rows on 4,096 shared and 256 own keys 48 us with the merge, 159 MB of keys and values (24 us at the
-// copy rate); 16 rows of 40 heads on 32,000 + 500 keys 47 us (22 us); 64 rows on 8,192 + 1,000 keys 54 us (25 us); 4 rows on 512 + 48 keys 15 us
-// (calls that read so little run row by row instead, in 8: ops.CudaOps.SHARED_BYTES).
+// copy rate); 16 rows of 40 heads on 32,000 + 500 keys 47 us (22 us); 64 rows on 8,192 + 1,000 keys 53 us (25 us); 4 rows on 512 + 48 keys 15 us
+// (calls that read so little run row by row instead, in 8: ops.CudaOps.SHARED_BYTES).  With heads of 64 the first takes 36 us (79 MB: 12 us), 64 rows 46, 16 rows of 32 heads 33:
+// a tile's softmax is the same, and its keys half as long.
 // Every block spends 4 us before its first tile (the lists, then the page table, then keys: three trips to memory one behind the other) and the merge is 6 to 9 us;
 // between them a tile takes an SM 1,850 clocks, memory alone would take 1,400: scores, softmax and weighted sum of a tile wait for one another, and two
 // blocks an SM (all that 102 KB of shared memory leave room for) do not quite hide it.  The tensor pipe is busy for 24 % of the time, DRAM for 50 %.

@@ -754,7 +754,7 @@ class CudaOps:
     # What the rows would read one by one, from which on sharing is the faster way: less stays in the L2 cache from one row to the next, and one launch does for it.
     # Microseconds, sharing / one by one, 32 heads over 8 of 128.  bfloat16: 4 rows x 512 keys 15 / 8, 16 x 1,024 (69 MB) 18 / 17, 8 x 2,048 (68 MB) 22 / 17, 8 x 4,096
     # (135 MB) 25 / 26, 16 x 2,048 (136 MB) 19 / 26, 8 groups of 4 x 1,024 (138 MB) 24 / 25, 8 x 8 x 1,024 (277 MB) 30 / 47, 8 x 8 x 4,096 46 / 157.  float32, whose
-    # multiply-adds bound the shared form: 13 rows x 1,600 (171 MB) 37 / 31, 8 x 4,096 (270 MB) 44 / 44, 8 x 8 x 512 (285 MB) 75 / 49, 16 x 4,096 (541 MB) 68 / 78, 8 x 8 x
+    # multiply-adds bound the shared form: 13 rows x 1,600 (171 MB) 37 / 29, 8 x 4,096 (270 MB) 44 / 44, 8 x 8 x 512 (285 MB) 75 / 49, 16 x 4,096 (541 MB) 68 / 78, 8 x 8 x
     # 2,048 (1.1 GB) 137 / 175.  It is no rule for many short prefixes, which stay in L2: 4 x 16 x 1,024 (545 MB) 92 / 79, 8 x 16 x 512 (570 MB) 126 / 97.
     SHARED_BYTES = {torch.bfloat16: 128 << 20, torch.float32: 512 << 20}
     # ... and how much of the longest row the longest shared prefix is at least, where the host says so (max_shared_len).  float32 tails fill an eighth of a tile's rows and
